@@ -311,6 +311,89 @@ int q27b_gemm_fp4_glu(int M, int I, int K, const uint8_t* a, const uint8_t* a_sf
  * board's power cap). The fused gather never uses it. */
 int q27b_quad_available(void);
 
+/* ---- between the q | k | v projection and the output projection -------------------------------------------------- */
+
+#define Q27B_F32 0
+#define Q27B_BF16 1
+#define Q27B_F16 2
+
+/* HOST function: the rotation speeds of rot_dim / 2 channel pairs, w_i = base^(-2 i / rot_dim) radians per position, as
+ * 64-bit binary fractions of a turn (turns[i] = round(2^64 w_i / 2 pi)), so that position * turns[i] modulo 2^64 is the
+ * angle modulo a turn at any position; and the factor on cos and sin. The caller copies turns to the device. scaling:
+ *   0 none;
+ *   1 linear: w_i / factor;
+ *   2 ntk: the base raised to base * factor^(rot_dim / (rot_dim - 2));
+ *   3 yarn (Peng et al. 2023): w_i where a pair turns more than beta_fast times over original_len positions, w_i / factor
+ *     where it turns less than beta_slow times, a ramp linear in the number of turns between; amplitude 0.1 ln(factor) + 1
+ *     (1 in the other cases). */
+int q27b_rope_turns(int rot_dim, double base, int scaling, double factor, double original_len, double beta_fast, double beta_slow,
+                    uint64_t* turns, float* amplitude);
+
+/* Queries and keys of T tokens: per-head RMS norm (when the weights are not null), rotation by position, and keys (and
+ * values, copied) into the paged cache or k_out. Strides in elements; channels of a head are contiguous. Bases and strides
+ * in whole groups of four channels. Outputs may be the inputs themselves (same type, base and strides), not otherwise
+ * overlap them. Beside rmsnorm_quant (the norm over the hidden size); the reference fuses the same steps into its
+ * attention's preparation kernel. */
+typedef struct q27b_qk_rope {
+  int T, q_heads, k_heads;     /* k_heads may be 0: queries only */
+  int head_dim, rot_dim;       /* multiples of 8; rot_dim <= head_dim <= 256: channels past rot_dim are not rotated */
+  int interleaved;             /* pairs (2 i, 2 i + 1) instead of (i, i + rot_dim / 2) */
+  int in_dtype, out_dtype;     /* Q27B_F32 / _BF16 / _F16 of q, k, v and of every output */
+  int pos64;                   /* positions are int64, else int32; negative positions rotate backwards */
+  int weight_f32;              /* norm weights are fp32, else bf16 */
+  int zero_centred;            /* the norm multiplies by 1 + w instead of w */
+  float eps, amplitude;        /* amplitude: the factor on cos and sin */
+  const void* positions;       /* [T] */
+  const uint64_t* turns;       /* [rot_dim / 2], device */
+  const void* q_weight;        /* [head_dim] or null: no norm */
+  const void* k_weight;
+  const void* q; int64_t q_ld_token, q_ld_head;
+  const void* k; int64_t k_ld_token, k_ld_head;
+  const void* v; int64_t v_ld_token, v_ld_head;          /* or null; k_heads heads; only with slots */
+  void* q_out; int64_t q_out_ld_token, q_out_ld_head;
+  void* k_out; int64_t k_out_ld_token, k_out_ld_head;    /* without slots */
+  const int64_t* slots;        /* [T] or null: place page * page_size + offset of each token in the cache; negative: the
+                                  token is not written; past the cache: not written, device status 9. Each at most once. */
+  int page_size, pages;
+  void* k_cache; int64_t kc_ld_page, kc_ld_head, kc_ld_slot;
+  void* v_cache; int64_t vc_ld_page, vc_ld_head, vc_ld_slot;
+} q27b_qk_rope;
+int q27b_qk_norm_rope(const q27b_qk_rope* args, void* stream);
+
+/* Attention of the newest tokens of B sequences over their keys and values in a paged cache, grouped queries (heads a
+ * multiple of kv_heads). Sequence b has kv_lens[b] tokens in the cache; its rows q_begin[b] .. q_begin[b + 1] of q are the
+ * newest of them. The token at position p sees the positions j <= p with j > p - window (window > 0) or j < sinks; a token
+ * that sees nothing (a negative position: more rows than tokens) gives zeros and an lse of -infinity. Rows of q in no
+ * sequence are left as they were. Pages that no row sees are never read and may hold any table entry; what lies in
+ * the cache behind a sequence's end is never used, whatever it holds. Strides in elements; channels contiguous; bases
+ * 16-byte aligned and strides multiples of 8 elements. Lengths, tables and rows may change between replays of a captured
+ * launch: the kernels read them on the device. A table entry that a row needs but that lies outside the cache, or a length
+ * past the table, reads nothing and raises device status 10. */
+typedef struct q27b_attention {
+  int dtype;                   /* Q27B_BF16 or Q27B_F16: q, cache and out */
+  int B, T;                    /* sequences; rows of q */
+  int heads, kv_heads, head_dim; /* head_dim 64, 128 or 256 */
+  int page_size, pages;        /* tokens per page: 16, 32, 64 or 128 */
+  int table_width;             /* table entries per sequence */
+  int window, sinks;           /* window 0: none */
+  int max_new, max_kv;         /* hints for the split of the work, at least 1: rows and length of the longest sequence. The
+                                  results hold whatever they say. */
+  float scale;                 /* on q . k */
+  int64_t table_ld;
+  const int32_t* table;        /* [B][table_width] */
+  const int32_t* kv_lens;      /* [B] */
+  const int32_t* q_begin;      /* [B + 1], or null: one row per sequence (T = B) */
+  const void* q; int64_t q_ld_token, q_ld_head;
+  const void* k_cache; int64_t kc_ld_page, kc_ld_head, kc_ld_slot;
+  const void* v_cache; int64_t vc_ld_page, vc_ld_head, vc_ld_slot;
+  void* out; int64_t out_ld_token, out_ld_head;
+  float* lse;                  /* [T][heads] natural logarithm of the sum of exp(scale q . k) over what the row sees, or null */
+  void* ws; size_t ws_bytes;   /* scratch of one call, any contents; not shared by calls that may overlap */
+} q27b_attention;
+/* Bytes of scratch that a call with these sizes needs (0: none). Reads no pointer of args. */
+int q27b_attention_workspace(const q27b_attention* args, size_t* bytes);
+int q27b_paged_attention(const q27b_attention* args, void* stream);
+
 /* Synchronises the device, returns and clears the status word kernels set when a bounded wait runs out
  * (0 = none; codes in csrc/ptx_sm100.cuh). No counterpart in the reference, whose kernels wait unboundedly. */
 int q27b_device_status(uint32_t* status);

@@ -20,6 +20,8 @@ enum : uint32_t {
   kStatusProbeTimeout = 6,       // the self-test's wait on a barrier nothing arrives at ran out, as it must
   kStatusTileWaitTimeout = 7,    // grouped launch: the pieces of a cut tile never all arrived
   kStatusPeerWaitTimeout = 8,    // fused gather: a peer GPU never reported its block of the outputs
+  kStatusBadSlot = 9,            // a cache slot past the cache's end: the token was not written
+  kStatusBadPage = 10,           // a page of the block table outside the cache, or a length past the table: not read
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

@@ -58,6 +58,10 @@ SIGNATURES = {
     "q27b_gemm_fp4_bf16": ([I, I, I, P, P, P, P, F, P, P], I),
     "q27b_gemm_fp4_glu_bf16": ([I, I, I, P, P, P, P, F, F, P, P], I),
     "q27b_gemm_fp4_glu": ([I, I, I, P, P, P, P, F, F, F, P, P, P], I),
+    "q27b_rope_turns": ([I, ctypes.c_double, I, ctypes.c_double, ctypes.c_double, ctypes.c_double, ctypes.c_double, P, P], I),
+    "q27b_qk_norm_rope": ([P, P], I),
+    "q27b_attention_workspace": ([P, P], I),
+    "q27b_paged_attention": ([P, P], I),
     "q27b_device_status": ([U32P], I),
     "q27b_quad_available": ([], I),
     "q27t_last_us": ([], F),
