@@ -4,6 +4,9 @@
 // Mathematics. Row i of a sequence with n new rows and L tokens stands at position p = L - n + i and sees the keys
 // j <= p with j > p - window or j < sinks. With s_j = scale q . k_j:  o = sum_j exp(s_j - m) v_j / l,  l = sum_j exp(s_j - m),
 // m the running maximum: one pass over the keys, in fp32.
+#include <algorithm>
+
+#include <cuda.h>
 #include <cuda_fp16.h>
 
 #include "../../include/q27b200/capi.h"
@@ -37,94 +40,84 @@ __device__ __forceinline__ Sequence sequence_of(const Args& p, int b) {
   return s;
 }
 
-// One warp per (row, head), keys one after the other.
-template <typename T2, int D>
-__global__ void __launch_bounds__(128) attention_row_kernel(const __grid_constant__ Args p, uint32_t* status) {
-  pdl_wait();
-  pdl_trigger();
-  const int64_t w = int64_t(blockIdx.x) * 4 + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (w >= int64_t(p.T) * p.heads) return;
-  const int t = int(w / p.heads), h = int(w % p.heads), hk = h / (p.heads / p.kv_heads);
-  int b = t;
-  if (p.q_begin) {  // the last b with q_begin[b] <= t
-    int lo = 0, hi = p.B;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (p.q_begin[mid] <= t) lo = mid + 1; else hi = mid;
-    }
-    b = lo - 1;
+// One row's result from its sums: D / N channels by each of N threads, 1 / l applied and rounded once; thread 0 the lse.
+template <typename T2, int D, int N>
+__device__ __forceinline__ void store_row(const Args& p, int t, int head, int part, float m, float l, const float* src) {
+  constexpr int E = D / N >= 8 ? 8 : D / N;
+  const bool some = !(l == 0.f);  // (NaN counts as something)
+  const float inv = some ? 1.f / l : 0.f;
+  uint16_t* out = static_cast<uint16_t*>(p.out) + t * p.out_ld_token + head * p.out_ld_head;
+#pragma unroll
+  for (int k = 0; k < D / (N * E); k++) {
+    const int d = (k * N + part) * E;
+    T2 w[E / 2];
+#pragma unroll
+    for (int e = 0; e < E / 2; e++) narrow(make_float2(src[d + 2 * e] * inv, src[d + 2 * e + 1] * inv), &w[e]);
+    if constexpr (E == 8)
+      *reinterpret_cast<uint4*>(out + d) = *reinterpret_cast<uint4*>(w);
+    else if constexpr (E == 4)
+      *reinterpret_cast<uint2*>(out + d) = *reinterpret_cast<uint2*>(w);
+    else
+      *reinterpret_cast<uint32_t*>(out + d) = *reinterpret_cast<uint32_t*>(w);
   }
-  if (b < 0 || b >= p.B) return;
-  const Sequence s = sequence_of(p, b);
-  if (t < s.row0 || t >= s.row0 + s.rows) return;
-  const int pos = s.len - s.rows + (t - s.row0);
-  constexpr int E = D / 64;  // channel pairs per lane
-  using Pair = T2;
-  float2 q[E], o[E];
-  const Pair* qp = reinterpret_cast<const Pair*>(static_cast<const uint16_t*>(p.q) + t * p.q_ld_token + h * p.q_ld_head);
-#pragma unroll
-  for (int e = 0; e < E; e++) q[e] = widen(qp[lane + 32 * e]), o[e] = make_float2(0.f, 0.f);
-  float m = -INFINITY, l = 0.f;
-  const int low = p.window > 0 ? max(pos - p.window + 1, 0) : 0;
-  const int end = min(pos + 1, s.reach);
-  if (pos + 1 > s.reach && lane == 0) atomicCAS(status, 0u, uint32_t(kStatusBadPage));
-  for (int j = 0; j < end; j++) {
-    if (j >= p.sinks && j < low) {
-      j = low - 1;
-      continue;
-    }
-    const int page = p.table[b * p.table_ld + j / p.page_size];
-    if (page < 0 || page >= p.pages) {
-      if (lane == 0) atomicCAS(status, 0u, uint32_t(kStatusBadPage));
-      continue;
-    }
-    const int at = j % p.page_size;
-    const Pair* kp = reinterpret_cast<const Pair*>(static_cast<const uint16_t*>(p.k_cache) + page * p.kc_ld_page + hk * p.kc_ld_head + at * p.kc_ld_slot);
-    const Pair* vp = reinterpret_cast<const Pair*>(static_cast<const uint16_t*>(p.v_cache) + page * p.vc_ld_page + hk * p.vc_ld_head + at * p.vc_ld_slot);
-    float d = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const float2 k = widen(kp[lane + 32 * e]);
-      d = fmaf(q[e].x, k.x, fmaf(q[e].y, k.y, d));
-    }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-    d *= p.scale;
-    const float m2 = fmaxf(m, d), keep = expf(m - m2), pr = expf(d - m2);
-    m = m2, l = l * keep + pr;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const float2 v = widen(vp[lane + 32 * e]);
-      o[e].x = o[e].x * keep + pr * v.x, o[e].y = o[e].y * keep + pr * v.y;
-    }
-  }
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  Pair* op = reinterpret_cast<Pair*>(static_cast<uint16_t*>(p.out) + t * p.out_ld_token + h * p.out_ld_head);
-#pragma unroll
-  for (int e = 0; e < E; e++) narrow(make_float2(o[e].x * inv, o[e].y * inv), &op[lane + 32 * e]);
-  if (p.lse && lane == 0) p.lse[w] = l > 0.f || l != l ? m + logf(l) : -INFINITY;
+  if (p.lse && part == 0) p.lse[int64_t(t) * p.heads + head] = some ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
 }
 
-template <typename T2, int D>
-int launch_rows(const Args& p, cudaStream_t s) {
-  uint32_t* status = device_status_ptr();
-  Q27B_REQUIRE(status, "attention: no device status word");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned((int64_t(p.T) * p.heads + 3) / 4)), cfg.blockDim = dim3(128), cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  Q27B_CUDA(cudaLaunchKernelEx(&cfg, attention_row_kernel<T2, D>, p, status));
+// ---- tensor maps -----------------------------------------------------------------------------------------------------
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  return fn;
+}
+
+// Keys or values as (channel, token in page, head, page), copied in boxes of 64 channels x `box` tokens with the 128-byte
+// swizzle; a page outside the cache reads as zeros.
+int make_cache_map(CUtensorMap* map, const Args& p, const void* cache, int64_t ld_page, int64_t ld_head, int64_t ld_slot, int box) {
+  EncodeTiledFn fn = encode_fn();
+  Q27B_REQUIRE(fn, "cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint64_t dims[4] = {cuuint64_t(p.head_dim), cuuint64_t(p.page_size), cuuint64_t(p.kv_heads), cuuint64_t(p.pages)};
+  const cuuint64_t row = cuuint64_t(p.head_dim) * 2;  // (the stride of a dimension of one is never used)
+  const cuuint64_t strides[3] = {cuuint64_t(ld_slot) * 2, p.kv_heads > 1 ? cuuint64_t(ld_head) * 2 : row, p.pages > 1 ? cuuint64_t(ld_page) * 2 : row};
+  const cuuint32_t boxes[4] = {64u, cuuint32_t(box), 1u, 1u}, estr[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = fn(map, p.dtype == Q27B_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(cache),
+                        dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  Q27B_REQUIRE(r == CUDA_SUCCESS, "attention: cuTensorMapEncodeTiled failed (%d) for cache strides %lld, %lld, %lld", int(r), (long long)ld_page,
+               (long long)ld_head, (long long)ld_slot);
   return 0;
 }
 
+#include "attention_stream.inl"
+
+template <typename T2, int D>
+int run(const Args& p, cudaStream_t s) {
+  uint32_t* status = device_status_ptr();
+  Q27B_REQUIRE(status, "attention: no device status word");
+  return launch_stream<T2, D>(p, 1 << 30, p.ws, s, status);
+}
+
 template <typename T2>
-int launch_dim(const Args& p, cudaStream_t s) {
-  if (p.head_dim == 64) return launch_rows<T2, 64>(p, s);
-  if (p.head_dim == 128) return launch_rows<T2, 128>(p, s);
-  return launch_rows<T2, 256>(p, s);
+int run_dim(const Args& p, cudaStream_t s) {
+  if (p.head_dim == 64) return run<T2, 64>(p, s);
+  if (p.head_dim == 128) return run<T2, 128>(p, s);
+  return run<T2, 256>(p, s);
+}
+
+size_t scratch_bytes(const Args& p) {
+  const int sms = sm_count();
+  if (p.head_dim == 64) return stream_scratch_bytes<64>(StreamCfg<64>::kCtasPerSm * sms);
+  if (p.head_dim == 128) return stream_scratch_bytes<128>(StreamCfg<128>::kCtasPerSm * sms);
+  return stream_scratch_bytes<256>(StreamCfg<256>::kCtasPerSm * sms);
 }
 
 int check_sizes(const Args& p) {
@@ -137,6 +130,7 @@ int check_sizes(const Args& p) {
                "attention: page_size must be 16, 32, 64 or 128 (%d)", p.page_size);
   Q27B_REQUIRE(p.pages > 0 && p.table_width > 0 && int64_t(p.table_width) * p.page_size < (int64_t(1) << 30),
                "attention: the cache and the table must not be empty, nor the table name 2^30 tokens or more (pages = %d, width = %d)", p.pages, p.table_width);
+  Q27B_REQUIRE(int64_t(p.T) * p.heads < (int64_t(1) << 30), "attention: T x heads must stay below 2^30 (%d, %d)", p.T, p.heads);
   Q27B_REQUIRE(p.window >= 0 && p.sinks >= 0, "attention: window and sinks must not be negative");
   Q27B_REQUIRE(p.max_new >= 1 && p.max_kv >= 1, "attention: max_new and max_kv must be at least 1");
   return 0;
@@ -155,13 +149,13 @@ extern "C" {
 int q27b_attention_workspace(const q27b_attention* a, size_t* bytes) {
   Q27B_REQUIRE(a && bytes, "attention_workspace: null arguments");
   if (int rc = check_sizes(*a)) return rc;
-  *bytes = 0;
+  *bytes = a->T == 0 || a->B == 0 ? 0 : scratch_bytes(*a);
   return 0;
 }
 
 int q27b_paged_attention(const q27b_attention* a, void* stream) {
   Q27B_REQUIRE(a, "attention: null arguments");
-  const Args& p = *a;
+  Args p = *a;
   if (int rc = check_sizes(p)) return rc;
   if (p.T == 0 || p.B == 0) return 0;
   Q27B_REQUIRE(p.q_begin || p.T == p.B, "attention: without q_begin there is one row per sequence (T = %d, B = %d)", p.T, p.B);
@@ -170,8 +164,13 @@ int q27b_paged_attention(const q27b_attention* a, void* stream) {
                "attention: q and out must not be null, 16-byte aligned, with strides that are multiples of 8 elements");
   Q27B_REQUIRE(rows16(p.k_cache, p.kc_ld_page, p.kc_ld_head, p.kc_ld_slot) && rows16(p.v_cache, p.vc_ld_page, p.vc_ld_head, p.vc_ld_slot),
                "attention: the cache must not be null, 16-byte aligned, with strides that are multiples of 8 elements");
+  Q27B_REQUIRE((p.kv_heads == 1 || (p.kc_ld_head > 0 && p.vc_ld_head > 0)) && (p.pages == 1 || (p.kc_ld_page > 0 && p.vc_ld_page > 0)) && p.kc_ld_slot > 0 && p.vc_ld_slot > 0,
+               "attention: the cache's strides must be positive");
+  const size_t need = scratch_bytes(p);
+  Q27B_REQUIRE(p.ws && (reinterpret_cast<uintptr_t>(p.ws) & 255u) == 0 && p.ws_bytes >= need, "attention: needs %zu bytes of 256-byte aligned scratch, got %zu", need, p.ws_bytes);
+  if (p.window >= (1 << 30)) p.window = 0;  // (no table names a position that far)
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return p.dtype == Q27B_BF16 ? launch_dim<__nv_bfloat162>(p, s) : launch_dim<__half2>(p, s);
+  return p.dtype == Q27B_BF16 ? run_dim<__nv_bfloat162>(p, s) : run_dim<__half2>(p, s);
 }
 
 }  // extern "C"
