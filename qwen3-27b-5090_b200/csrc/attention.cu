@@ -98,12 +98,29 @@ int make_cache_map(CUtensorMap* map, const Args& p, const void* cache, int64_t l
 }
 
 #include "attention_stream.inl"
+#include "attention_tile.inl"
+
+// Which kernels a call needs: sequences of up to kStreamRows query rows per key head stream, longer ones go through the tensor
+// cores' 128-row tiles. The host knows the rows only through the hint, so whichever kernels it picks take every sequence between
+// them: a kernel that is alone takes all.
+struct Choice {
+  bool stream, tile;
+};
+Choice choose(const Args& p) {
+  const int64_t rows = int64_t(p.q_begin ? std::min(p.max_new, p.T) : 1) * (p.heads / p.kv_heads);
+  const bool tile = rows > kStreamRows;
+  return {!tile || (p.B > 1 && p.heads / p.kv_heads <= kStreamRows && p.q_begin), tile};
+}
 
 template <typename T2, int D>
 int run(const Args& p, cudaStream_t s) {
   uint32_t* status = device_status_ptr();
   Q27B_REQUIRE(status, "attention: no device status word");
-  return launch_stream<T2, D>(p, 1 << 30, p.ws, s, status);
+  const Choice c = choose(p);
+  if (c.stream)
+    if (int rc = launch_stream<T2, D>(p, c.tile ? kStreamRows : 1 << 30, p.ws, s, status)) return rc;
+  if (c.tile) return launch_tile<T2, D>(p, c.stream ? kStreamRows + 1 : 1, p.ws, s, status);
+  return 0;
 }
 
 template <typename T2>
@@ -113,11 +130,17 @@ int run_dim(const Args& p, cudaStream_t s) {
   return run<T2, 256>(p, s);
 }
 
-size_t scratch_bytes(const Args& p) {
+// (the two kernels of a mixed call run one after the other: they share the scratch)
+template <int D>
+size_t scratch_bytes_of(const Args& p) {
+  const Choice c = choose(p);
   const int sms = sm_count();
-  if (p.head_dim == 64) return stream_scratch_bytes<64>(StreamCfg<64>::kCtasPerSm * sms);
-  if (p.head_dim == 128) return stream_scratch_bytes<128>(StreamCfg<128>::kCtasPerSm * sms);
-  return stream_scratch_bytes<256>(StreamCfg<256>::kCtasPerSm * sms);
+  return std::max(c.stream ? stream_scratch_bytes<D>(StreamCfg<D>::kCtasPerSm * sms) : size_t(0), c.tile ? tile_scratch_bytes<D>(sms) : size_t(0));
+}
+size_t scratch_bytes(const Args& p) {
+  if (p.head_dim == 64) return scratch_bytes_of<64>(p);
+  if (p.head_dim == 128) return scratch_bytes_of<128>(p);
+  return scratch_bytes_of<256>(p);
 }
 
 int check_sizes(const Args& p) {

@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(kStreamThreads, StreamCfg<D>::kCtasPerSm)
     const uint32_t box_bytes = uint32_t(box) * 128u;         // per 64 channels
     int stage = 0, issued = 0;
     uint32_t phase = 0;
+    bool stop = false;  // a wait ran out (the same in all lanes)
     int held_b = -1, held_from = 0, held = 0, ahead = 0;  // page-table entries, one per lane: 32 from held_from, and the next 32
     for (int64_t t = t0; t < t1 && cur.b < p.B; cur.next(p, max_rows)) {
       const StreamSeq& q = cur.q;
@@ -188,8 +189,10 @@ __global__ void __launch_bounds__(kStreamThreads, StreamCfg<D>::kCtasPerSm)
       const int reach = min(q.s.len, q.s.reach);
       for (; cur.i < end; cur.i++, t++) {
         const int key0 = q.tile(cur.i) * kStreamKeys;
-        if (issued >= C::kStages) warp_wait(empty(stage), phase ^ 1u, &abort_flag, status, kStatusEmptyWaitTimeout, 0);
-        if (abort_flag) break;
+        if (issued >= C::kStages && !warp_wait(empty(stage), phase ^ 1u, &abort_flag, status, kStatusEmptyWaitTimeout, 0)) {
+          stop = true;
+          break;
+        }
         uint32_t bytes = 0;
         int page_at[4] = {};
         bool need[4];
@@ -234,9 +237,9 @@ __global__ void __launch_bounds__(kStreamThreads, StreamCfg<D>::kCtasPerSm)
         if (++stage == C::kStages) stage = 0, phase ^= 1u;
       }
       if (cur.b < p.B && q.s.len > q.s.reach && lane == 0) atomicCAS(status, 0u, uint32_t(kStatusBadPage));
-      if (abort_flag) break;
+      if (stop) break;
     }
-    if (abort_flag) {  // unwinding: no copy may still be in flight when the CTA ends
+    if (stop) {  // unwinding: no copy may still be in flight when the CTA ends
       for (int s = 0; s < C::kStages && s < issued; s++) {
         const int last = issued - 1 - ((issued - 1 - s) % C::kStages + C::kStages) % C::kStages;  // last use of ring place s
         uint32_t unused = 0;
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kStreamThreads, StreamCfg<D>::kCtasPerSm)
     float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
 
     for (int i = from; i < end; i++, t++) {
-      const bool here = !abort_flag && warp_wait(full(stage), phase, &abort_flag, status, kStatusFullWaitTimeout, 0);
+      const bool here = warp_wait(full(stage), phase, &abort_flag, status, kStatusFullWaitTimeout, 0);
       const int k0 = q.tile(i) * kStreamKeys + my_key, k1 = k0 + 15;  // this warp's keys
       const bool some = k0 <= pmax && k0 < reach && (p.window == 0 || k1 > pmin - p.window || k0 < p.sinks);
       if (here && some) {

@@ -1,0 +1,670 @@
+// Prompts and chunks: many query rows per key head. The tensor cores bound it (and, close behind, the exponentials). Included
+// by attention.cu.
+//
+// Work. The query rows of one key head (row = token x heads per key head: the heads of a group share their keys, so a tile of 128
+// rows spans few positions and little of it is masked) are cut into segments of kTiles x 128 rows; a segment's work is
+// its 128-key tiles, from the window and the sinks of its first row to the position of its last. As in the streaming kernel
+// all segments' tiles are cut into equal ranges, one per SM, and the pieces of cut segments joined afterwards.
+//
+// Arithmetic, per 128-row tile: S = Q K^T by tcgen05.mma into tensor memory; a warpgroup with one thread per row reads its row
+// of S, takes the running maximum, writes P = 2^(c s - c m) back over S in the inputs' type, and O += P V follows with P as the
+// tensor-memory operand and V straight from its row-major tile (the transposed shared-memory operand form). O stays in tensor
+// memory; it is scaled down only when a row's maximum has grown by more than 8 binary orders since the last time (P then
+// stays below 2^8, exact to the same relative step), so that most tiles skip the round trip. Up to 128 channels two
+// row tiles take turns: while one's softmax runs, the other's products do. At 256 channels O of one tile fills half the tensor
+// memory; there is one row tile, with two S buffers.
+//
+// Roles: one warpgroup per row tile (softmax, scaling, epilogue, and the load of the next segment's Q), one thread that issues the
+// products, one warp that issues the copies. K and V pass through one ring in the order in which the products use them.
+
+template <int D>
+struct TileCfg {
+  static constexpr int kTiles = D == 256 ? 1 : 2;                // row tiles of a segment
+  static constexpr int kRows = 128 * kTiles;
+  static constexpr int kKeys = 128;
+  static constexpr int kParts = D == 256 ? 2 : 1;                // ring slots per K or V tile
+  static constexpr int kSlotBytes = kKeys * D * 2 / kParts;
+  static constexpr int kSlots = D == 64 ? 8 : 4;
+  static constexpr int kQBytes = 128 * D * 2;
+  static constexpr int kSoftmaxWarps = 4 * kTiles;
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
+  static constexpr int kSmemBytes = 1024 + kTiles * kQBytes + kSlots * kSlotBytes + 256;
+  static constexpr int kPieceFloats = kRows * (D + 2);
+  static constexpr int kO = 256;                                 // tensor-memory column of the (first) output; S at 0 and 128
+};
+
+__device__ __forceinline__ int tile_of(int i, int sink_tiles, int first_window_tile) { return i < sink_tiles ? i : first_window_tile + i - sink_tiles; }
+
+// The key tiles that rows [row0, row1) of a sequence see (row = token x G).
+struct TileRange {
+  int low, reach;  // window start of the first row; keys [0, reach) can be seen by the last row
+  int sink_tiles, first_window_tile, tiles;
+  int pmin, pmax;
+};
+__device__ __forceinline__ TileRange tile_range(const Args& p, const Sequence& s, int G, int row0, int row1) {
+  TileRange r;
+  const int first = s.len - s.rows;
+  r.pmin = first + row0 / G, r.pmax = first + (row1 - 1) / G;
+  r.reach = max(min(r.pmax + 1, s.reach), 0);
+  r.low = p.window > 0 ? max(r.pmin - p.window + 1, 0) : 0;
+  r.sink_tiles = (min(min(p.sinks, r.low), r.reach) + 127) / 128;
+  r.first_window_tile = max(r.low / 128, r.sink_tiles);
+  r.tiles = max(r.sink_tiles + max((r.reach + 127) / 128 - r.first_window_tile, 0), 1);
+  return r;
+}
+
+__device__ __forceinline__ int heavy_rows(const Args& p, const Sequence& s, int min_rows) {
+  const int rows = s.rows * (p.heads / p.kv_heads);
+  return rows >= min_rows ? rows : 0;
+}
+
+struct TileCursor {
+  int b, hk, rt, i, rows;  // rows of the sequence; i: tile within the segment
+  Sequence s;
+  TileRange r;
+  template <int kRows>
+  __device__ void load(const Args& p) {
+    r = tile_range(p, s, p.heads / p.kv_heads, rt * kRows, min((rt + 1) * kRows, rows));
+  }
+  template <int kRows>
+  __device__ void next(const Args& p, int min_rows) {
+    i = 0;
+    if (++rt * kRows >= rows) {
+      rt = 0;
+      if (++hk >= p.kv_heads) {
+        hk = 0;
+        do {
+          if (++b >= p.B) return;
+          s = sequence_of(p, b), rows = heavy_rows(p, s, min_rows);
+        } while (rows == 0);
+      }
+    }
+    load<kRows>(p);
+  }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+      "%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+      "%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem]^T and D[tmem] (+)= A[tmem] B[smem]; one thread issues.
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor of kind::f16: fp32 accumulator, both operands bf16 or both fp16, A K-major, 128 x n x 16.
+__host__ __device__ constexpr uint32_t umma_idesc_f16(bool bf16, bool b_mn_major, uint32_t n) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// Shared-memory descriptor of an operand whose rows are K (keys) and whose 64-channel blocks of 128-byte rows carry the 128-byte
+// swizzle: blocks `block_bytes` apart along N, groups of 8 keys 1024 bytes apart along K.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t block_bytes) {
+  return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(block_bytes >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+
+template <typename T2>
+struct is_bf16 { static constexpr bool value = false; };
+template <>
+struct is_bf16<__nv_bfloat162> { static constexpr bool value = true; };
+
+template <typename T2, int D>
+__global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
+    attention_tile_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                          const __grid_constant__ Args p, int min_rows, int box, float* pieces, JoinRecord* records, uint32_t* status) {
+  using C = TileCfg<D>;
+  constexpr int NT = C::kTiles;
+  extern __shared__ uint8_t raw[];
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t ring = base + NT * C::kQBytes;
+  __shared__ uint64_t bars[2 * C::kSlots + 9];
+  __shared__ volatile uint32_t abort_flag;
+  __shared__ uint32_t tmem_word;
+  __shared__ int64_t sums[12];
+  __shared__ int64_t start_off;
+  __shared__ int start_b, start_rt, start_i;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  constexpr int kWarps = C::kThreads / 32;
+  auto full = [&](int s) { return smem_u32(bars + s); };
+  auto empty = [&](int s) { return smem_u32(bars + C::kSlots + s); };
+  auto s_full = [&](int t) { return smem_u32(bars + 2 * C::kSlots + t); };
+  auto p_ready = [&](int t) { return smem_u32(bars + 2 * C::kSlots + 2 + t); };
+  auto q_ready = [&](int t) { return smem_u32(bars + 2 * C::kSlots + 4 + t); };
+  auto pv_done = [&](int t) { return smem_u32(bars + 2 * C::kSlots + 6 + t); };
+  const uint32_t drained = smem_u32(bars + 2 * C::kSlots + 8);
+
+  if (tid == 0) {
+    abort_flag = 0, start_b = -1;
+    for (int s = 0; s < C::kSlots; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+    for (int t = 0; t < 2; t++) mbar_init(s_full(t), 1), mbar_init(p_ready(t), 128), mbar_init(q_ready(t), 128), mbar_init(pv_done(t), 1);
+    mbar_init(drained, 1);
+    mbar_init_fence();
+    prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- this CTA's range of the tiles: every warp sums a run of sequences, its lanes share a sequence's segments ---------------
+  const int G = p.heads / p.kv_heads, run = (p.B + kWarps - 1) / kWarps, b_lo = min(warp * run, p.B), b_hi = min(b_lo + run, p.B);
+  auto tiles_of = [&](const Sequence& s, int rows) {  // tiles of all segments of one key head, over the lanes
+    int n = 0;
+    for (int rt = lane; rt * C::kRows < rows; rt += 32) n += tile_range(p, s, G, rt * C::kRows, min((rt + 1) * C::kRows, rows)).tiles;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+  };
+  auto each_heavy = [&](auto&& f) {  // f(b, sequence, rows) for the warp's sequences that this kernel takes
+    for (int b0 = b_lo; b0 < b_hi; b0 += 32) {
+      const int b = b0 + lane;
+      Sequence s = {};
+      int rows = 0;
+      if (b < b_hi) s = sequence_of(p, b), rows = heavy_rows(p, s, min_rows);
+      for (uint32_t left = __ballot_sync(0xffffffffu, rows > 0); left; left &= left - 1) {
+        const int from = __ffs(left) - 1;
+        Sequence u;
+        u.row0 = __shfl_sync(0xffffffffu, s.row0, from), u.rows = __shfl_sync(0xffffffffu, s.rows, from);
+        u.len = __shfl_sync(0xffffffffu, s.len, from), u.reach = __shfl_sync(0xffffffffu, s.reach, from);
+        f(b0 + from, u, __shfl_sync(0xffffffffu, rows, from));
+      }
+    }
+  };
+  int64_t mine = 0;
+  each_heavy([&](int, const Sequence& s, int rows) { mine += int64_t(p.kv_heads) * tiles_of(s, rows); });
+  if (lane == 0) sums[warp] = mine;
+  __syncthreads();
+  int64_t total = 0, before = 0;
+  for (int w = 0; w < kWarps; w++) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  const int64_t ctas = min(int64_t(gridDim.x), total), c = blockIdx.x;
+  if (c >= ctas) {
+    if (tid == 0) records[c].pieces = 0;
+    return;
+  }
+  const int64_t t0 = total * c / ctas, t1 = total * (c + 1) / ctas;
+  if (before <= t0 && t0 < before + mine) {
+    each_heavy([&](int b, const Sequence& s, int rows) {
+      const int n = tiles_of(s, rows);
+      const int64_t w = int64_t(p.kv_heads) * n;
+      if (before <= t0 && t0 < before + w) {
+        int off = int((t0 - before) % n);  // among one key head's tiles
+        int acc = 0;
+        for (int r0 = 0; r0 * C::kRows < rows; r0 += 32) {
+          const int rt = r0 + lane;
+          const int m = rt * C::kRows < rows ? tile_range(p, s, G, rt * C::kRows, min((rt + 1) * C::kRows, rows)).tiles : 0;
+          int upto = m;
+#pragma unroll
+          for (int o = 1; o < 32; o *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+          }
+          if (m > 0 && acc + upto - m <= off && off < acc + upto) start_b = b, start_off = (t0 - before) / n, start_rt = rt, start_i = off - (acc + upto - m);
+          acc += __shfl_sync(0xffffffffu, upto, 31);
+        }
+      }
+      before += w;
+    });
+  }
+  if (warp == 0) {  // (after the exit above: what is taken is given back)
+    tmem_alloc(smem_u32(&tmem_word), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_word;
+  TileCursor cur;
+  cur.b = start_b;
+  const bool work = cur.b >= 0;  // (false: the lengths changed under the kernel)
+  if (work) {
+    cur.s = sequence_of(p, cur.b), cur.rows = heavy_rows(p, cur.s, min_rows);
+    cur.hk = int(start_off), cur.rt = start_rt;
+    cur.template load<C::kRows>(p);
+    cur.i = start_i;
+  }
+  if (tid == 0) {
+    JoinRecord r = {0, cur.b, cur.hk, cur.rt};
+    if (work) {
+      const int64_t s0 = t0 - cur.i, s1 = s0 + cur.r.tiles;
+      if (cur.i > 0 && total * (c - 1) / ctas <= s0) r.pieces = int((s1 * ctas + total - 1) / total - 1 - c) + 2;
+    }
+    records[c] = r;
+  }
+
+  if (warp == C::kSoftmaxWarps + 1) {
+    // ---- copies -----------------------------------------------------------------------------------------------------------
+    const int boxes = C::kKeys / box;  // per tile: at most eight, one per lane
+    int slot = 0, issued = 0;
+    uint32_t phase = 0;
+    bool stop = false;  // a wait ran out (the same in all lanes)
+    auto load = [&](const CUtensorMap* map, bool values, int i) {  // all lanes
+      if (stop) return;
+      const int tile0 = tile_of(i, cur.r.sink_tiles, cur.r.first_window_tile) * C::kKeys;
+      const int k0 = tile0 + lane * box, k1 = min(k0 + box, cur.r.reach);
+      const bool need = lane < boxes && k0 < cur.r.reach && (k0 < p.sinks || k1 > cur.r.low);  // pages that no row sees are not read
+      int page = 0;
+      if (need) {
+        page = p.table[cur.b * p.table_ld + k0 / p.page_size];
+        if (page < 0 || page >= p.pages) page = p.pages, atomicCAS(status, 0u, uint32_t(kStatusBadPage));  // (reads zeros)
+      }
+      const uint32_t needs = __ballot_sync(0xffffffffu, need);
+#pragma unroll
+      for (int part = 0; part < C::kParts; part++) {
+        // K is split along its channels, V along its keys
+        const uint32_t in_part = C::kParts == 1 || !values ? needs : needs & (((1u << (boxes / 2)) - 1u) << (part * (boxes / 2)));
+        constexpr int kBlocks = D / 64;
+        const int d0 = C::kParts == 2 && !values ? part * kBlocks / 2 : 0, dn = C::kParts == 2 && !values ? kBlocks / 2 : kBlocks;
+        const int rows = C::kParts == 2 && values ? C::kKeys / 2 : C::kKeys;
+        if (issued >= C::kSlots && !warp_wait(empty(slot), phase ^ 1u, &abort_flag, status, kStatusEmptyWaitTimeout, 0)) {
+          stop = true;
+          return;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(full(slot), uint32_t(__popc(in_part) * dn * box) * 128u);
+        __syncwarp();
+        if ((in_part >> lane) & 1u) {
+          const uint32_t dst = ring + slot * C::kSlotBytes + uint32_t((k0 - tile0) - (rows < C::kKeys ? part * rows : 0)) * 128u;
+          for (int d = 0; d < dn; d++) tma_load_4d(dst + d * rows * 128, map, (d0 + d) * 64, k0 % p.page_size, cur.hk, page, full(slot));
+        }
+        issued++;
+        if (++slot == C::kSlots) slot = 0, phase ^= 1u;
+      }
+    };
+    if (work)
+      for (int64_t t = t0; t < t1 && cur.b < p.B && !stop; cur.template next<C::kRows>(p, min_rows)) {
+        const int from = cur.i, end = int(min(int64_t(cur.r.tiles), from + (t1 - t)));
+        if (cur.s.len > cur.s.reach && lane == 0) atomicCAS(status, 0u, uint32_t(kStatusBadPage));
+        load(&kmap, false, from);
+        for (int i = from; i < end; i++) {  // the order in which the products use them
+          if (NT == 1 && i + 1 < end) load(&kmap, false, i + 1);
+          load(&vmap, true, i);
+          if (NT == 2 && i + 1 < end) load(&kmap, false, i + 1);
+        }
+        t += end - from;
+      }
+    if (stop)  // unwinding: no copy may still be in flight when the CTA ends
+      for (int s = 0; s < C::kSlots && s < issued; s++) {
+        const int last = issued - 1 - ((issued - 1 - s) % C::kSlots + C::kSlots) % C::kSlots;  // last use of slot s
+        uint32_t unused = 0;
+        if (lane == 0) mbar_wait_bounded(full(s), uint32_t(last / C::kSlots) & 1u, &abort_flag, &unused, kStatusDrainTimeout);
+      }
+  } else if (warp == C::kSoftmaxWarps) {
+    // ---- products ---------------------------------------------------------------------------------------------------------
+    if (lane == 0 && work) {
+      constexpr uint32_t qk_idesc = umma_idesc_f16(is_bf16<T2>::value, false, C::kKeys), pv_idesc = umma_idesc_f16(is_bf16<T2>::value, true, D);
+      int slot = 0;
+      uint32_t phase = 0, p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) {
+        ok = ok && !abort_flag && mbar_wait_bounded(bar, parity, &abort_flag, status, code);
+        tc_fence_after_sync();
+      };
+      auto advance = [&](int& s, uint32_t& ph) { if (++s == C::kSlots) s = 0, ph ^= 1u; };
+      // S of row tile t (buffer `buf`) from the K tile at ring place (s, ph); waits for the copies
+      auto qk = [&](int t, int buf, int s, uint32_t ph) {
+        for (int part = 0; part < C::kParts; part++) {
+          wait(full(s), ph, kStatusFullWaitTimeout);
+          if (!ok) return;
+          const uint32_t kb = ring + s * C::kSlotBytes, qb = base + t * C::kQBytes + part * (C::kQBytes / C::kParts);
+#pragma unroll
+          for (int k = 0; k < D / 16 / C::kParts; k++)
+            umma_f16_ss(tmem + buf * 128, umma_desc_k_sw128(qb + (k / 4) * 128 * 128 + (k % 4) * 32), umma_desc_k_sw128(kb + (k / 4) * C::kKeys * 128 + (k % 4) * 32),
+                        qk_idesc, part + k > 0);
+          if (C::kParts > 1) umma_commit(empty(s));
+          advance(s, ph);
+        }
+      };
+      auto pv = [&](int t, int buf, int s, uint32_t ph, bool accumulate) {
+        for (int part = 0; part < C::kParts; part++) {
+          wait(full(s), ph, kStatusFullWaitTimeout);
+          if (!ok) return;
+          const uint32_t vb = ring + s * C::kSlotBytes;
+          constexpr int kPartKeys = C::kKeys / C::kParts;
+#pragma unroll
+          for (int k = 0; k < kPartKeys / 16; k++)
+            umma_f16_ts(tmem + C::kO + t * D, tmem + buf * 128 + part * (kPartKeys / 2) + k * 8, umma_desc_mn_sw128(vb + k * 2048, kPartKeys * 128), pv_idesc,
+                        accumulate || part + k > 0);
+          if (C::kParts > 1) umma_commit(empty(s));
+          advance(s, ph);
+        }
+      };
+      auto skip = [&](int parts) { for (int i = 0; i < parts; i++) advance(slot, phase); };
+      for (int64_t t = t0; t < t1 && cur.b < p.B && ok; cur.template next<C::kRows>(p, min_rows)) {
+        const int from = cur.i, end = int(min(int64_t(cur.r.tiles), from + (t1 - t)));
+        t += end - from;
+        const int active = min(C::kRows, cur.rows - cur.rt * C::kRows) > 128 ? 2 : 1;
+        for (int x = 0; x < active; x++) wait(q_ready(x), q_phase[x], kStatusAccumWaitTimeout), q_phase[x] ^= 1u;
+        if constexpr (NT == 2) {
+          for (int x = 0; x < active && ok; x++) qk(x, x, slot, phase), umma_commit(s_full(x));
+          if (!ok) break;
+          umma_commit(empty(slot));
+          skip(1);
+          for (int i = from; i < end && ok; i++) {
+            const int vs = slot;
+            const uint32_t vp = phase;
+            skip(1);
+            const bool more = i + 1 < end;
+            for (int x = 0; x < active && ok; x++) {
+              wait(p_ready(x), p_phase[x], kStatusAccumWaitTimeout), p_phase[x] ^= 1u;
+              if (!ok) break;
+              pv(x, x, vs, vp, i > from);
+              if (x == active - 1 && ok) umma_commit(empty(vs));
+              if (!ok) break;
+              if (more) {
+                qk(x, x, slot, phase);
+                if (!ok) break;
+                umma_commit(s_full(x));
+                if (x == active - 1) umma_commit(empty(slot));
+              } else {
+                umma_commit(pv_done(x));
+              }
+            }
+            if (more) skip(1);
+          }
+        } else {
+          int buf = 0;  // of the tile whose P comes next
+          qk(0, 0, slot, phase);
+          if (!ok) break;
+          umma_commit(s_full(0));
+          skip(C::kParts);
+          for (int i = from; i < end && ok; i++) {
+            if (i + 1 < end) {
+              qk(0, buf ^ 1, slot, phase);
+              if (!ok) break;
+              umma_commit(s_full(buf ^ 1));
+              skip(C::kParts);
+            }
+            wait(p_ready(buf), p_phase[buf], kStatusAccumWaitTimeout), p_phase[buf] ^= 1u;
+            if (!ok) break;
+            pv(0, buf, slot, phase, i > from);
+            if (!ok) break;
+            umma_commit(pv_done(0));
+            skip(C::kParts);
+            buf ^= 1;
+          }
+          // the next segment starts at buffer 0 again
+        }
+      }
+      umma_commit(drained);  // no product may be in flight when the tensor memory is given back, after a failed wait either
+      uint32_t unused = 0;
+      mbar_wait_bounded(drained, 0, &unused, nullptr, kStatusDrainTimeout);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax, scaling, epilogue: one thread per row ---------------------------------------------------------------------
+    const int tile = warp / 4, row_in_tile = tid % 128;
+    const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16;
+    const float c2 = fabsf(p.scale) * 1.4426950408889634f, scale_log2 = c2 > 0.f ? c2 : 1e-30f;  // (0 would turn a masked -infinity into NaN)
+    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale goes into the queries' signs
+    uint32_t s_phase[2] = {0, 0}, pv_phase = 0;
+    int chunk = 0;  // ring places used before this segment
+    // this thread's row of the segment at `at` into shared memory, in the layout of the products' operands
+    auto load_q = [&](const TileCursor& at) {
+      const int row = at.rt * C::kRows + tile * 128 + row_in_tile;
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + (at.s.row0 + row / G) * p.q_ld_token + (at.hk * G + row % G) * p.q_ld_head;
+      const uint32_t dst = base + tile * C::kQBytes + row_in_tile * 128;
+      const bool live = row < at.rows;
+#pragma unroll
+      for (int d = 0; d < D / 8; d++) {
+        uint4 v = live ? reinterpret_cast<const uint4*>(src)[d] : make_uint4(0, 0, 0, 0);
+        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (d / 8) * 128 * 128 + (((d % 8) ^ (row_in_tile & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(q_ready(tile));
+    };
+    auto in_use = [&](const TileCursor& at) { return at.rows - at.rt * C::kRows > tile * 128; };
+    if (work && in_use(cur)) load_q(cur);
+    for (int64_t t = t0; work && t < t1 && cur.b < p.B;) {
+      const int from = cur.i, end = int(min(int64_t(cur.r.tiles), from + (t1 - t)));
+      t += end - from;
+      TileCursor nxt = cur;
+      nxt.template next<C::kRows>(p, min_rows);
+      const bool more = t < t1 && nxt.b < p.B;
+      if (in_use(cur)) {
+        const int row = cur.rt * C::kRows + tile * 128 + row_in_tile, row_end = min(cur.rows, cur.rt * C::kRows + tile * 128 + 128);
+        const int first = cur.s.len - cur.s.rows, pos = first + row / G;
+        const int tile_pmin = first + (cur.rt * C::kRows + tile * 128) / G, tile_pmax = first + (row_end - 1) / G;
+        const bool warp_live = cur.rt * C::kRows + tile * 128 + (warp % 4) * 32 < cur.rows;  // a warp without rows only keeps step
+        float m = -INFINITY, l = 0.f;
+        for (int i = from; i < end; i++) {
+          const int buf = NT == 2 ? tile : (i - from) & 1;
+          const uint32_t s_at = tmem + lanes + buf * 128;
+          const int k0 = tile_of(i, cur.r.sink_tiles, cur.r.first_window_tile) * C::kKeys, k1 = k0 + C::kKeys - 1;
+          const bool here = !abort_flag && mbar_wait_bounded(s_full(buf), s_phase[buf], &abort_flag, status, kStatusAccumWaitTimeout);
+          s_phase[buf] ^= 1u;
+          if (!__all_sync(0xffffffffu, here)) continue;
+          tc_fence_after_sync();
+          auto wait_pv = [&] {  // of the tile before (kTiles == 1): it may still be adding to O
+            mbar_wait_bounded(pv_done(0), pv_phase ^ 1u, &abort_flag, status, kStatusAccumWaitTimeout);
+            tc_fence_after_sync();
+          };
+          if (warp_live) {
+            float s[128];
+#pragma unroll
+            for (int x = 0; x < 4; x++) tmem_ld32(s_at + 32 * x, s + 32 * x);
+            tmem_ld_wait();
+            const bool all = k1 <= tile_pmin && k1 < cur.r.reach && (p.window == 0 || k0 > tile_pmax - p.window || k1 < p.sinks);
+            if (!all) {
+              const int hi = min(pos, cur.r.reach - 1) - k0, lo = p.window > 0 ? pos - p.window + 1 - k0 : -1, si = p.sinks - k0;
+#pragma unroll
+              for (int x = 0; x < 128; x++) s[x] = x <= hi && (x >= lo || x < si) ? s[x] : -INFINITY;
+            }
+            float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int x = 4; x < 128; x++) top[x & 3] = fmaxf(top[x & 3], s[x]);
+            const float tile_m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            const bool grow = m == -INFINITY ? tile_m > m : (tile_m - m) * scale_log2 > 8.f;
+            if (__any_sync(0xffffffffu, grow)) {
+              const float f = grow ? exp2_fast((m - tile_m) * scale_log2) : 1.f;  // (m = -infinity: 0)
+              if (grow) m = tile_m, l *= f;
+              if (i > from) {
+                if (NT == 1) wait_pv();
+#pragma unroll
+                for (int d = 0; d < D; d += 32) {
+                  float o[32];
+                  tmem_ld32(tmem + lanes + C::kO + tile * D + d, o);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int x = 0; x < 32; x++) o[x] *= f;
+                  tmem_st32(tmem + lanes + C::kO + tile * D + d, reinterpret_cast<uint32_t*>(o));
+                }
+              }
+            }
+            const float mc = m == -INFINITY ? 0.f : m * scale_log2;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              uint32_t w[32];
+#pragma unroll
+              for (int x = 0; x < 32; x++) {
+                const float a = exp2_fast(fmaf(s[64 * h + 2 * x], scale_log2, -mc)), b = exp2_fast(fmaf(s[64 * h + 2 * x + 1], scale_log2, -mc));
+                sum[(2 * x) & 3] += a, sum[(2 * x + 1) & 3] += b;
+                T2 v;
+                narrow(make_float2(a, b), &v);
+                w[x] = *reinterpret_cast<uint32_t*>(&v);
+              }
+              tmem_st32(s_at + 32 * h, w);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st_wait();
+          }
+          if (NT == 1) {
+            // The product of the tile before is awaited in every turn, whether O was scaled or not: were it left running, its phase and
+            // that of this tile's product could not be told apart.
+            if (i > from) wait_pv();
+            pv_phase ^= 1u;
+          }
+          // Values of keys that no row of the segment sees are whatever the cache (or an earlier tile) left there, and 0 x NaN would be
+          // NaN: the first warpgroup, whose P every product waits for, clears them.
+          if (tile == 0 && !(k1 <= cur.r.pmin && k1 < cur.r.reach && (p.window == 0 || k0 > cur.r.pmin - p.window || k1 < p.sinks))) {
+            const int key = k0 + row_in_tile;
+            const bool any = key < cur.r.reach && (p.window == 0 || key > cur.r.pmin - p.window || key < p.sinks);
+            const int n = end - from, j = i - from;
+            int at = chunk + (NT == 2 ? 2 * j + 1 : C::kParts * min(2 * j + 2, 2 * n - 1));  // ring place of this V tile
+            constexpr int kPartKeys = C::kKeys / C::kParts;
+            at += row_in_tile / kPartKeys;
+            if (!any) {
+              mbar_wait_bounded(full(at % C::kSlots), uint32_t(at / C::kSlots) & 1u, &abort_flag, status, kStatusFullWaitTimeout);
+              const uint32_t dst = ring + (at % C::kSlots) * C::kSlotBytes + (row_in_tile % kPartKeys) * 128;
+#pragma unroll
+              for (int d = 0; d < D / 64; d++)
+#pragma unroll
+                for (int x = 0; x < 8; x++)
+                  asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst + d * kPartKeys * 128 + x * 16), "r"(0) : "memory");
+              fence_proxy_async_smem();
+            }
+          }
+          tc_fence_before_sync();
+          mbar_arrive(p_ready(buf));
+        }
+        // every product with this segment's Q has ended (its S was read): the next segment's may take its place
+        if (more && in_use(nxt)) load_q(nxt);
+        // the last product of the segment, then its result
+        const bool done = !abort_flag && mbar_wait_bounded(pv_done(tile), NT == 2 ? pv_phase : pv_phase ^ 1u, &abort_flag, status, kStatusAccumWaitTimeout);
+        if (NT == 2) pv_phase ^= 1u;
+        if (__all_sync(0xffffffffu, done) && warp_live) {
+          tc_fence_after_sync();
+          const bool whole = from == 0 && end == cur.r.tiles, live = row < cur.rows;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          uint16_t* out = static_cast<uint16_t*>(p.out) + (cur.s.row0 + row / G) * p.out_ld_token + (cur.hk * G + row % G) * p.out_ld_head;
+          float* piece = pieces + (2 * c + (from > 0 ? 0 : 1)) * C::kPieceFloats;
+#pragma unroll
+          for (int d = 0; d < D; d += 32) {
+            float o[32];
+            tmem_ld32(tmem + lanes + C::kO + tile * D + d, o);
+            tmem_ld_wait();
+            if (whole && live) {
+#pragma unroll
+              for (int x = 0; x < 32; x += 8) {
+                T2 w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) narrow(make_float2(o[x + 2 * e] * inv, o[x + 2 * e + 1] * inv), &w[e]);
+                *reinterpret_cast<uint4*>(out + d + x) = *reinterpret_cast<uint4*>(w);
+              }
+            }
+            if (!whole && live) {  // channel groups of four, rows side by side: a warp's stores are contiguous
+#pragma unroll
+              for (int x = 0; x < 32; x += 4)
+                *reinterpret_cast<float4*>(piece + ((d + x) / 4 * C::kRows + tile * 128 + row_in_tile) * 4) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+            }
+          }
+          const float mb = m * scale_log2;  // (-infinity stays)
+          if (whole && live && p.lse) p.lse[int64_t(cur.s.row0 + row / G) * p.heads + cur.hk * G + row % G] = l == 0.f ? -INFINITY : (mb + log2f(l)) * 0.6931471805599453f;
+          if (!whole && live) piece[C::kRows * D + tile * 128 + row_in_tile] = mb, piece[C::kRows * (D + 1) + tile * 128 + row_in_tile] = l;
+          tc_fence_before_sync();
+        }
+      } else if (more && in_use(nxt)) {
+        load_q(nxt);
+      }
+      chunk += 2 * (end - from) * C::kParts;
+      cur = nxt;
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// Joins the pieces of the cut segments: block (c, y, z) takes 128 rows and 32 channels of the segment whose first cut is the
+// start of CTA c's range.
+template <typename T2, int D>
+__global__ void __launch_bounds__(128) attention_tile_join_kernel(const __grid_constant__ Args p, const float* pieces, const JoinRecord* records) {
+  using C = TileCfg<D>;
+  pdl_wait();
+  pdl_trigger();
+  const int c = blockIdx.x, in_seg = blockIdx.y * 128 + threadIdx.x, d0 = blockIdx.z * 32;
+  const JoinRecord r = records[c];
+  if (r.pieces == 0) return;
+  const Sequence s = sequence_of(p, r.b);
+  const int G = p.heads / p.kv_heads, row = r.rg * C::kRows + in_seg;
+  if (row >= s.rows * G) return;
+  auto piece = [&](int i) { return pieces + int64_t(i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i)) * C::kPieceFloats; };
+  float m = -INFINITY, l = 0.f;
+  for (int i = 0; i < r.pieces; i++) m = fmaxf(m, piece(i)[C::kRows * D + in_seg]);
+  float4 o[8] = {};
+  for (int i = 0; i < r.pieces; i++) {
+    const float* x = piece(i);
+    const float mi = x[C::kRows * D + in_seg], f = mi == -INFINITY ? 0.f : exp2_fast(mi - m);
+    l += f * x[C::kRows * (D + 1) + in_seg];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float4 v = *reinterpret_cast<const float4*>(x + ((d0 / 4 + e) * C::kRows + in_seg) * 4);
+      o[e].x += f * v.x, o[e].y += f * v.y, o[e].z += f * v.z, o[e].w += f * v.w;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* out = static_cast<uint16_t*>(p.out) + (s.row0 + row / G) * p.out_ld_token + (r.hk * G + row % G) * p.out_ld_head + d0;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    T2 w[4];
+    narrow(make_float2(o[e].x * inv, o[e].y * inv), &w[0]), narrow(make_float2(o[e].z * inv, o[e].w * inv), &w[1]);
+    narrow(make_float2(o[e + 1].x * inv, o[e + 1].y * inv), &w[2]), narrow(make_float2(o[e + 1].z * inv, o[e + 1].w * inv), &w[3]);
+    *reinterpret_cast<uint4*>(out + 4 * e) = *reinterpret_cast<uint4*>(w);
+  }
+  if (p.lse && blockIdx.z == 0) p.lse[int64_t(s.row0 + row / G) * p.heads + r.hk * G + row % G] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <int D>
+size_t tile_scratch_bytes(int ctas) {
+  return (size_t(ctas) * sizeof(JoinRecord) + 255) / 256 * 256 + size_t(ctas) * 2 * TileCfg<D>::kPieceFloats * 4;
+}
+
+template <typename T2, int D>
+int launch_tile(const Args& p, int min_rows, void* ws, cudaStream_t s, uint32_t* status) {
+  using C = TileCfg<D>;
+  auto kernel = attention_tile_kernel<T2, D>;
+  static bool done[64] = {};
+  int dev = 0;
+  Q27B_CUDA(cudaGetDevice(&dev));
+  if (!(dev < 64 && done[dev])) {
+    Q27B_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    if (dev < 64) done[dev] = true;
+  }
+  CUtensorMap km, vm;
+  const int box = std::min(p.page_size, C::kKeys / C::kParts);
+  if (int rc = make_cache_map(&km, p, p.k_cache, p.kc_ld_page, p.kc_ld_head, p.kc_ld_slot, box)) return rc;
+  if (int rc = make_cache_map(&vm, p, p.v_cache, p.vc_ld_page, p.vc_ld_head, p.vc_ld_slot, box)) return rc;
+  const int ctas = sm_count();
+  JoinRecord* records = static_cast<JoinRecord*>(ws);
+  float* pieces = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + (size_t(ctas) * sizeof(JoinRecord) + 255) / 256 * 256);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(ctas)), cfg.blockDim = dim3(C::kThreads), cfg.dynamicSmemBytes = C::kSmemBytes, cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 1 : 0;
+  Q27B_CUDA(cudaLaunchKernelEx(&cfg, kernel, km, vm, p, min_rows, box, pieces, records, status));
+  cfg.gridDim = dim3(unsigned(ctas), C::kTiles, D / 32), cfg.blockDim = dim3(128), cfg.dynamicSmemBytes = 0;
+  Q27B_CUDA(cudaLaunchKernelEx(&cfg, attention_tile_join_kernel<T2, D>, p, static_cast<const float*>(pieces), static_cast<const JoinRecord*>(records)));
+  return 0;
+}
