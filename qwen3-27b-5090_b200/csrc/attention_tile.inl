@@ -22,12 +22,19 @@ struct TileCfg {
   static constexpr int kTiles = D == 256 ? 1 : 2;                // row tiles of a segment
   static constexpr int kRows = 128 * kTiles;
   static constexpr int kKeys = 128;
+  // What a segment costs beside its tiles (Q, the start and the end of the pipeline, the epilogue), in tiles: it counts in the shares
+  static constexpr int kSegmentCost = 3;
   static constexpr int kParts = D == 256 ? 2 : 1;                // ring slots per K or V tile
   static constexpr int kSlotBytes = kKeys * D * 2 / kParts;
   static constexpr int kSlots = D == 64 ? 8 : 4;
   static constexpr int kQBytes = 128 * D * 2;
   static constexpr int kSoftmaxWarps = 4 * kTiles;
-  static constexpr int kThreads = 32 * (kSoftmaxWarps + 2);
+  // whole warpgroups where registers are moved between them (two warps idle)
+  static constexpr int kThreads = kTiles == 2 ? 384 : 32 * (kSoftmaxWarps + 2);
+  // Two row tiles: 384 threads get 168 registers each at launch; the softmax keeps a row of S in registers and takes 200, the
+  // others go down to 104: 2 x 128 x 200 + 128 x 104 = 384 x 168, never more than the launch got.
+  static constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
+  static_assert(kTiles == 1 || 256 * kSoftmaxRegs + 128 * kOtherRegs <= 384 * kLaunchRegs, "registers");
   static constexpr int kSmemBytes = 1024 + kTiles * kQBytes + kSlots * kSlotBytes + 256;
   static constexpr int kPieceFloats = kRows * (D + 2);
   static constexpr int kO = 256;                                 // tensor-memory column of the (first) output; S at 0 and 128
@@ -59,16 +66,19 @@ __device__ __forceinline__ int heavy_rows(const Args& p, const Sequence& s, int 
 }
 
 struct TileCursor {
-  int b, hk, rt, i, rows;  // rows of the sequence; i: tile within the segment
+  int b, hk, rt, from, rows;  // rows of the sequence; from: this CTA's first tile of the segment
+  int64_t at;                 // where the segment's tiles begin in the order of all shares (its own cost lies before them)
   Sequence s;
   TileRange r;
+  __device__ int end(int64_t t1) const { return int(max(int64_t(0), min(int64_t(r.tiles), t1 - at))); }  // of a range up to t1
+  __device__ bool any(const Args& p, int64_t t1) const { return b < p.B && from < end(t1); }
   template <int kRows>
   __device__ void load(const Args& p) {
     r = tile_range(p, s, p.heads / p.kv_heads, rt * kRows, min((rt + 1) * kRows, rows));
   }
-  template <int kRows>
+  template <int kRows, int kCost>
   __device__ void next(const Args& p, int min_rows) {
-    i = 0;
+    from = 0, at += r.tiles + kCost;
     if (++rt * kRows >= rows) {
       rt = 0;
       if (++hk >= p.kv_heads) {
@@ -87,6 +97,21 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -153,6 +178,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   __shared__ int start_b, start_rt, start_i;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   constexpr int kWarps = C::kThreads / 32;
+  static_assert(kWarps <= 12, "sums");
   auto full = [&](int s) { return smem_u32(bars + s); };
   auto empty = [&](int s) { return smem_u32(bars + C::kSlots + s); };
   auto s_full = [&](int t) { return smem_u32(bars + 2 * C::kSlots + t); };
@@ -174,9 +200,9 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
 
   // ---- this CTA's range of the tiles: every warp sums a run of sequences, its lanes share a sequence's segments ---------------
   const int G = p.heads / p.kv_heads, run = (p.B + kWarps - 1) / kWarps, b_lo = min(warp * run, p.B), b_hi = min(b_lo + run, p.B);
-  auto tiles_of = [&](const Sequence& s, int rows) {  // tiles of all segments of one key head, over the lanes
+  auto cost_of = [&](const Sequence& s, int rows) {  // of all segments of one key head, over the lanes
     int n = 0;
-    for (int rt = lane; rt * C::kRows < rows; rt += 32) n += tile_range(p, s, G, rt * C::kRows, min((rt + 1) * C::kRows, rows)).tiles;
+    for (int rt = lane; rt * C::kRows < rows; rt += 32) n += C::kSegmentCost + tile_range(p, s, G, rt * C::kRows, min((rt + 1) * C::kRows, rows)).tiles;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
@@ -197,7 +223,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
     }
   };
   int64_t mine = 0;
-  each_heavy([&](int, const Sequence& s, int rows) { mine += int64_t(p.kv_heads) * tiles_of(s, rows); });
+  each_heavy([&](int, const Sequence& s, int rows) { mine += int64_t(p.kv_heads) * cost_of(s, rows); });
   if (lane == 0) sums[warp] = mine;
   __syncthreads();
   int64_t total = 0, before = 0;
@@ -213,14 +239,14 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   const int64_t t0 = total * c / ctas, t1 = total * (c + 1) / ctas;
   if (before <= t0 && t0 < before + mine) {
     each_heavy([&](int b, const Sequence& s, int rows) {
-      const int n = tiles_of(s, rows);
+      const int n = cost_of(s, rows);
       const int64_t w = int64_t(p.kv_heads) * n;
       if (before <= t0 && t0 < before + w) {
-        int off = int((t0 - before) % n);  // among one key head's tiles
+        int off = int((t0 - before) % n);  // among one key head's segments
         int acc = 0;
         for (int r0 = 0; r0 * C::kRows < rows; r0 += 32) {
           const int rt = r0 + lane;
-          const int m = rt * C::kRows < rows ? tile_range(p, s, G, rt * C::kRows, min((rt + 1) * C::kRows, rows)).tiles : 0;
+          const int m = rt * C::kRows < rows ? C::kSegmentCost + tile_range(p, s, G, rt * C::kRows, min((rt + 1) * C::kRows, rows)).tiles : 0;
           int upto = m;
 #pragma unroll
           for (int o = 1; o < 32; o *= 2) {
@@ -249,17 +275,21 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
     cur.s = sequence_of(p, cur.b), cur.rows = heavy_rows(p, cur.s, min_rows);
     cur.hk = int(start_off), cur.rt = start_rt;
     cur.template load<C::kRows>(p);
-    cur.i = start_i;
+    // (start_i: the position within the segment, its own cost first)
+    cur.from = max(start_i - C::kSegmentCost, 0), cur.at = t0 - start_i + C::kSegmentCost;
   }
   if (tid == 0) {
     JoinRecord r = {0, cur.b, cur.hk, cur.rt};
     if (work) {
-      const int64_t s0 = t0 - cur.i, s1 = s0 + cur.r.tiles;
-      if (cur.i > 0 && total * (c - 1) / ctas <= s0) r.pieces = int((s1 * ctas + total - 1) / total - 1 - c) + 2;
+      const int64_t s1 = cur.at + cur.r.tiles;
+      if (cur.from > 0 && total * (c - 1) / ctas <= cur.at) r.pieces = int((s1 * ctas + total - 1) / total - 1 - c) + 2;
     }
     records[c] = r;
   }
 
+  if (warp >= C::kSoftmaxWarps) {
+  if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+  // (two row tiles: two more warps, idle, complete the warpgroup)
   if (warp == C::kSoftmaxWarps + 1) {
     // ---- copies -----------------------------------------------------------------------------------------------------------
     const int boxes = C::kKeys / box;  // per tile: at most eight, one per lane
@@ -299,8 +329,8 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       }
     };
     if (work)
-      for (int64_t t = t0; t < t1 && cur.b < p.B && !stop; cur.template next<C::kRows>(p, min_rows)) {
-        const int from = cur.i, end = int(min(int64_t(cur.r.tiles), from + (t1 - t)));
+      for (; cur.any(p, t1) && !stop; cur.template next<C::kRows, C::kSegmentCost>(p, min_rows)) {
+        const int from = cur.from, end = cur.end(t1);
         if (cur.s.len > cur.s.reach && lane == 0) atomicCAS(status, 0u, uint32_t(kStatusBadPage));
         load(&kmap, false, from);
         for (int i = from; i < end; i++) {  // the order in which the products use them
@@ -308,7 +338,6 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
           load(&vmap, true, i);
           if (NT == 2 && i + 1 < end) load(&kmap, false, i + 1);
         }
-        t += end - from;
       }
     if (stop)  // unwinding: no copy may still be in flight when the CTA ends
       for (int s = 0; s < C::kSlots && s < issued; s++) {
@@ -357,9 +386,8 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
         }
       };
       auto skip = [&](int parts) { for (int i = 0; i < parts; i++) advance(slot, phase); };
-      for (int64_t t = t0; t < t1 && cur.b < p.B && ok; cur.template next<C::kRows>(p, min_rows)) {
-        const int from = cur.i, end = int(min(int64_t(cur.r.tiles), from + (t1 - t)));
-        t += end - from;
+      for (; cur.any(p, t1) && ok; cur.template next<C::kRows, C::kSegmentCost>(p, min_rows)) {
+        const int from = cur.from, end = cur.end(t1);
         const int active = min(C::kRows, cur.rows - cur.rt * C::kRows) > 128 ? 2 : 1;
         for (int x = 0; x < active; x++) wait(q_ready(x), q_phase[x], kStatusAccumWaitTimeout), q_phase[x] ^= 1u;
         if constexpr (NT == 2) {
@@ -418,7 +446,9 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       mbar_wait_bounded(drained, 0, &unused, nullptr, kStatusDrainTimeout);
     }
     __syncwarp();
+  }
   } else {
+    if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
     // ---- softmax, scaling, epilogue: one thread per row ---------------------------------------------------------------------
     const int tile = warp / 4, row_in_tile = tid % 128;
     const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16;
@@ -442,13 +472,13 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       mbar_arrive(q_ready(tile));
     };
     auto in_use = [&](const TileCursor& at) { return at.rows - at.rt * C::kRows > tile * 128; };
-    if (work && in_use(cur)) load_q(cur);
-    for (int64_t t = t0; work && t < t1 && cur.b < p.B;) {
-      const int from = cur.i, end = int(min(int64_t(cur.r.tiles), from + (t1 - t)));
-      t += end - from;
-      TileCursor nxt = cur;
-      nxt.template next<C::kRows>(p, min_rows);
-      const bool more = t < t1 && nxt.b < p.B;
+    if (work && cur.any(p, t1) && in_use(cur)) load_q(cur);
+    while (work && cur.any(p, t1)) {
+      const int from = cur.from, end = cur.end(t1);
+      auto load_next_q = [&](TileCursor nxt) {
+        nxt.template next<C::kRows, C::kSegmentCost>(p, min_rows);
+        if (nxt.any(p, t1) && in_use(nxt)) load_q(nxt);
+      };
       if (in_use(cur)) {
         const int row = cur.rt * C::kRows + tile * 128 + row_in_tile, row_end = min(cur.rows, cur.rt * C::kRows + tile * 128 + 128);
         const int first = cur.s.len - cur.s.rows, pos = first + row / G;
@@ -500,21 +530,24 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
               }
             }
             const float mc = m == -INFINITY ? 0.f : m * scale_log2;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const float2 scale2 = make_float2(scale_log2, scale_log2), off2 = make_float2(-mc, -mc);
+            float2 sum[2] = {};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
               uint32_t w[32];
 #pragma unroll
               for (int x = 0; x < 32; x++) {
-                const float a = exp2_fast(fmaf(s[64 * h + 2 * x], scale_log2, -mc)), b = exp2_fast(fmaf(s[64 * h + 2 * x + 1], scale_log2, -mc));
-                sum[(2 * x) & 3] += a, sum[(2 * x + 1) & 3] += b;
+                float2 e = fma2(make_float2(s[64 * h + 2 * x], s[64 * h + 2 * x + 1]), scale2, off2);
+                e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                sum[x & 1] = add2(sum[x & 1], e);
                 T2 v;
-                narrow(make_float2(a, b), &v);
+                narrow(e, &v);
                 w[x] = *reinterpret_cast<uint32_t*>(&v);
               }
               tmem_st32(s_at + 32 * h, w);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            sum[0] = add2(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
             tmem_st_wait();
           }
           if (NT == 1) {
@@ -547,7 +580,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
           mbar_arrive(p_ready(buf));
         }
         // every product with this segment's Q has ended (its S was read): the next segment's may take its place
-        if (more && in_use(nxt)) load_q(nxt);
+        load_next_q(cur);
         // the last product of the segment, then its result
         const bool done = !abort_flag && mbar_wait_bounded(pv_done(tile), NT == 2 ? pv_phase : pv_phase ^ 1u, &abort_flag, status, kStatusAccumWaitTimeout);
         if (NT == 2) pv_phase ^= 1u;
@@ -582,11 +615,11 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
           if (!whole && live) piece[C::kRows * D + tile * 128 + row_in_tile] = mb, piece[C::kRows * (D + 1) + tile * 128 + row_in_tile] = l;
           tc_fence_before_sync();
         }
-      } else if (more && in_use(nxt)) {
-        load_q(nxt);
+      } else {
+        load_next_q(cur);
       }
       chunk += 2 * (end - from) * C::kParts;
-      cur = nxt;
+      cur.template next<C::kRows, C::kSegmentCost>(p, min_rows);
     }
   }
   tc_fence_before_sync();
@@ -648,6 +681,11 @@ int launch_tile(const Args& p, int min_rows, void* ws, cudaStream_t s, uint32_t*
   Q27B_CUDA(cudaGetDevice(&dev));
   if (!(dev < 64 && done[dev])) {
     Q27B_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    if (C::kTiles == 2) {  // (a build that gave the launch fewer registers than the warpgroups then ask for would wait for them for ever)
+      cudaFuncAttributes attrs;
+      Q27B_CUDA(cudaFuncGetAttributes(&attrs, kernel));
+      Q27B_REQUIRE(attrs.numRegs >= C::kLaunchRegs, "attention: the kernel was built with %d registers instead of %d", attrs.numRegs, C::kLaunchRegs);
+    }
     if (dev < 64) done[dev] = true;
   }
   CUtensorMap km, vm;
