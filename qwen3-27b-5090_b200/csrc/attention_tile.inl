@@ -98,6 +98,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -190,7 +195,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   if (tid == 0) {
     abort_flag = 0, start_b = -1;
     for (int s = 0; s < C::kSlots; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
-    for (int t = 0; t < 2; t++) mbar_init(s_full(t), 1), mbar_init(p_ready(t), 128), mbar_init(q_ready(t), 128), mbar_init(pv_done(t), 1);
+    for (int t = 0; t < 2; t++) mbar_init(s_full(t), 1), mbar_init(p_ready(t), 4), mbar_init(q_ready(t), 128), mbar_init(pv_done(t), 1);
     mbar_init(drained, 1);
     mbar_init_fence();
     prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
@@ -346,102 +351,123 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
         if (lane == 0) mbar_wait_bounded(full(s), uint32_t(last / C::kSlots) & 1u, &abort_flag, &unused, kStatusDrainTimeout);
       }
   } else if (warp == C::kSoftmaxWarps) {
-    // ---- products ---------------------------------------------------------------------------------------------------------
-    if (lane == 0 && work) {
+    // ---- products -----------------------------------------------------------------------------------------------------------
+    // The whole warp walks the segments and waits, so that addresses and descriptors stay uniform; one elected lane issues. (A
+    // single-lane branch spent 115 cycles per product on moving descriptors, more than the products take.)
+    if (work) {
       constexpr uint32_t qk_idesc = umma_idesc_f16(is_bf16<T2>::value, false, C::kKeys), pv_idesc = umma_idesc_f16(is_bf16<T2>::value, true, D);
+      constexpr int kPartKeys = C::kKeys / C::kParts;
+      const uint64_t q_desc = umma_desc_k_sw128(base), k_desc = umma_desc_k_sw128(ring), v_desc = umma_desc_mn_sw128(ring, kPartKeys * 128);
       int slot = 0;
-      uint32_t phase = 0, p_phase[2] = {0, 0}, q_phase[2] = {0, 0};
+      uint32_t phase = 0, p_phase = 0, q_phase = 0;  // (bit t: of row tile or S buffer t)
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) {
-        ok = ok && !abort_flag && mbar_wait_bounded(bar, parity, &abort_flag, status, code);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(bar, parity, &abort_flag, status, code));
         tc_fence_after_sync();
       };
-      auto advance = [&](int& s, uint32_t& ph) { if (++s == C::kSlots) s = 0, ph ^= 1u; };
-      // S of row tile t (buffer `buf`) from the K tile at ring place (s, ph); waits for the copies
-      auto qk = [&](int t, int buf, int s, uint32_t ph) {
-        for (int part = 0; part < C::kParts; part++) {
-          wait(full(s), ph, kStatusFullWaitTimeout);
-          if (!ok) return;
-          const uint32_t kb = ring + s * C::kSlotBytes, qb = base + t * C::kQBytes + part * (C::kQBytes / C::kParts);
+      auto wait_p = [&](int t) { wait(p_ready(t), (p_phase >> t) & 1u, kStatusAccumWaitTimeout), p_phase ^= 1u << t; };
+      auto advance = [&] { if (++slot == C::kSlots) slot = 0, phase ^= 1u; };
+      // S of row tile t into buffer `buf` from the K part in ring slot s
+      auto qk_part = [&](int t, int buf, int s, int part) {
+        const uint64_t qd = q_desc + uint64_t((t * C::kQBytes + part * (C::kQBytes / C::kParts)) >> 4), kd = k_desc + uint64_t(s * (C::kSlotBytes >> 4));
+        const uint32_t d = tmem + buf * 128;
 #pragma unroll
-          for (int k = 0; k < D / 16 / C::kParts; k++)
-            umma_f16_ss(tmem + buf * 128, umma_desc_k_sw128(qb + (k / 4) * 128 * 128 + (k % 4) * 32), umma_desc_k_sw128(kb + (k / 4) * C::kKeys * 128 + (k % 4) * 32),
-                        qk_idesc, part + k > 0);
-          if (C::kParts > 1) umma_commit(empty(s));
-          advance(s, ph);
+        for (int k = 0; k < D / 16 / C::kParts; k++) {
+          const uint32_t off = ((k / 4) * C::kKeys * 128 + (k % 4) * 32) >> 4;  // (the rows of Q's blocks are as many as K's)
+          umma_f16_ss(d, qd + off, kd + off, qk_idesc, part + k > 0);
         }
       };
-      auto pv = [&](int t, int buf, int s, uint32_t ph, bool accumulate) {
-        for (int part = 0; part < C::kParts; part++) {
-          wait(full(s), ph, kStatusFullWaitTimeout);
-          if (!ok) return;
-          const uint32_t vb = ring + s * C::kSlotBytes;
-          constexpr int kPartKeys = C::kKeys / C::kParts;
+      auto pv_part = [&](int t, int buf, int s, int part, bool accumulate) {
+        const uint64_t vd = v_desc + uint64_t(s * (C::kSlotBytes >> 4));
+        const uint32_t d = tmem + C::kO + t * D, a = tmem + buf * 128 + part * (kPartKeys / 2);
 #pragma unroll
-          for (int k = 0; k < kPartKeys / 16; k++)
-            umma_f16_ts(tmem + C::kO + t * D, tmem + buf * 128 + part * (kPartKeys / 2) + k * 8, umma_desc_mn_sw128(vb + k * 2048, kPartKeys * 128), pv_idesc,
-                        accumulate || part + k > 0);
-          if (C::kParts > 1) umma_commit(empty(s));
-          advance(s, ph);
-        }
+        for (int k = 0; k < kPartKeys / 16; k++) umma_f16_ts(d, a + k * 8, vd + ((k * 2048) >> 4), pv_idesc, k > 0 || accumulate);
       };
-      auto skip = [&](int parts) { for (int i = 0; i < parts; i++) advance(slot, phase); };
       for (; cur.any(p, t1) && ok; cur.template next<C::kRows, C::kSegmentCost>(p, min_rows)) {
         const int from = cur.from, end = cur.end(t1);
         const int active = min(C::kRows, cur.rows - cur.rt * C::kRows) > 128 ? 2 : 1;
-        for (int x = 0; x < active; x++) wait(q_ready(x), q_phase[x], kStatusAccumWaitTimeout), q_phase[x] ^= 1u;
+        for (int x = 0; x < active; x++) wait(q_ready(x), (q_phase >> x) & 1u, kStatusAccumWaitTimeout), q_phase ^= 1u << x;
         if constexpr (NT == 2) {
-          for (int x = 0; x < active && ok; x++) qk(x, x, slot, phase), umma_commit(s_full(x));
+          wait(full(slot), phase, kStatusFullWaitTimeout);
           if (!ok) break;
-          umma_commit(empty(slot));
-          skip(1);
-          for (int i = from; i < end && ok; i++) {
-            const int vs = slot;
-            const uint32_t vp = phase;
-            skip(1);
+          if (elect_one()) {
+            for (int x = 0; x < active; x++) qk_part(x, x, slot, 0), umma_commit(s_full(x));
+            umma_commit(empty(slot));
+          }
+          __syncwarp();
+          advance();
+          for (int i = from; i < end; i++) {
             const bool more = i + 1 < end;
-            for (int x = 0; x < active && ok; x++) {
-              wait(p_ready(x), p_phase[x], kStatusAccumWaitTimeout), p_phase[x] ^= 1u;
-              if (!ok) break;
-              pv(x, x, vs, vp, i > from);
-              if (x == active - 1 && ok) umma_commit(empty(vs));
-              if (!ok) break;
+            const int vs = slot;
+            wait(full(slot), phase, kStatusFullWaitTimeout);  // V of this tile
+            advance();
+            wait_p(0);
+            if (more) wait(full(slot), phase, kStatusFullWaitTimeout);  // K of the next
+            if (!ok) break;
+            if (elect_one()) {
+              pv_part(0, 0, vs, 0, i > from);
+              if (active == 1) umma_commit(empty(vs));
               if (more) {
-                qk(x, x, slot, phase);
-                if (!ok) break;
-                umma_commit(s_full(x));
-                if (x == active - 1) umma_commit(empty(slot));
+                qk_part(0, 0, slot, 0);
+                umma_commit(s_full(0));
+                if (active == 1) umma_commit(empty(slot));
               } else {
-                umma_commit(pv_done(x));
+                umma_commit(pv_done(0));
               }
             }
-            if (more) skip(1);
+            __syncwarp();
+            if (active == 2) {
+              wait_p(1);
+              if (!ok) break;
+              if (elect_one()) {
+                pv_part(1, 1, vs, 0, i > from);
+                umma_commit(empty(vs));
+                if (more) {
+                  qk_part(1, 1, slot, 0);
+                  umma_commit(s_full(1));
+                  umma_commit(empty(slot));
+                } else {
+                  umma_commit(pv_done(1));
+                }
+              }
+              __syncwarp();
+            }
+            if (more) advance();
           }
         } else {
-          int buf = 0;  // of the tile whose P comes next
-          qk(0, 0, slot, phase);
-          if (!ok) break;
-          umma_commit(s_full(0));
-          skip(C::kParts);
-          for (int i = from; i < end && ok; i++) {
-            if (i + 1 < end) {
-              qk(0, buf ^ 1, slot, phase);
-              if (!ok) break;
-              umma_commit(s_full(buf ^ 1));
-              skip(C::kParts);
+          auto qk = [&](int buf) {
+            for (int part = 0; part < C::kParts && ok; part++) {
+              wait(full(slot), phase, kStatusFullWaitTimeout);
+              if (ok && elect_one()) {
+                qk_part(0, buf, slot, part);
+                umma_commit(empty(slot));
+                if (part == C::kParts - 1) umma_commit(s_full(buf));
+              }
+              __syncwarp();
+              advance();
             }
-            wait(p_ready(buf), p_phase[buf], kStatusAccumWaitTimeout), p_phase[buf] ^= 1u;
-            if (!ok) break;
-            pv(0, buf, slot, phase, i > from);
-            if (!ok) break;
-            umma_commit(pv_done(0));
-            skip(C::kParts);
+          };
+          int buf = 0;  // of the tile whose P comes next; every segment starts at 0
+          qk(0);
+          for (int i = from; i < end && ok; i++) {
+            if (i + 1 < end) qk(buf ^ 1);
+            wait_p(buf);
+            for (int part = 0; part < C::kParts && ok; part++) {
+              wait(full(slot), phase, kStatusFullWaitTimeout);
+              if (ok && elect_one()) {
+                pv_part(0, buf, slot, part, part > 0 || i > from);
+                umma_commit(empty(slot));
+                if (part == C::kParts - 1) umma_commit(pv_done(0));
+              }
+              __syncwarp();
+              advance();
+            }
             buf ^= 1;
           }
-          // the next segment starts at buffer 0 again
         }
       }
-      umma_commit(drained);  // no product may be in flight when the tensor memory is given back, after a failed wait either
+      if (elect_one()) umma_commit(drained);  // no product may be in flight when the tensor memory is given back, after a failed wait either
+      __syncwarp();
       uint32_t unused = 0;
       mbar_wait_bounded(drained, 0, &unused, nullptr, kStatusDrainTimeout);
     }
@@ -510,8 +536,9 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
             }
             float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int x = 4; x < 128; x++) top[x & 3] = fmaxf(top[x & 3], s[x]);
-            const float tile_m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            for (int x = 4; x < 124; x += 2) top[(x / 2) & 3] = max3(top[(x / 2) & 3], s[x], s[x + 1]);
+            top[0] = max3(top[0], s[124], s[125]), top[1] = max3(top[1], s[126], s[127]);
+            const float tile_m = fmaxf(max3(top[0], top[1], top[2]), top[3]);
             const bool grow = m == -INFINITY ? tile_m > m : (tile_m - m) * scale_log2 > 8.f;
             if (__any_sync(0xffffffffu, grow)) {
               const float f = grow ? exp2_fast((m - tile_m) * scale_log2) : 1.f;  // (m = -infinity: 0)
@@ -577,7 +604,8 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
             }
           }
           tc_fence_before_sync();
-          mbar_arrive(p_ready(buf));
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_ready(buf));
         }
         // every product with this segment's Q has ended (its S was read): the next segment's may take its place
         load_next_q(cur);
