@@ -24,17 +24,17 @@ struct TileCfg {
   static constexpr int kKeys = 128;
   // What a segment costs beside its tiles (Q, the start and the end of the pipeline, the epilogue), in tiles: it counts in the shares
   static constexpr int kSegmentCost = 3;
+  static constexpr int kPolyEvery = 3;                           // every third pair's exponentials on the FMA units
   static constexpr int kParts = D == 256 ? 2 : 1;                // ring slots per K or V tile
   static constexpr int kSlotBytes = kKeys * D * 2 / kParts;
   static constexpr int kSlots = D == 64 ? 8 : 4;
   static constexpr int kQBytes = 128 * D * 2;
-  static constexpr int kSoftmaxWarps = 4 * kTiles;
-  // whole warpgroups where registers are moved between them (two warps idle)
-  static constexpr int kThreads = kTiles == 2 ? 384 : 32 * (kSoftmaxWarps + 2);
-  // Two row tiles: 384 threads get 168 registers each at launch; the softmax keeps a row of S in registers and takes 200, the
-  // others go down to 104: 2 x 128 x 200 + 128 x 104 = 384 x 168, never more than the launch got.
-  static constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kOtherRegs = 72;
-  static_assert(kTiles == 1 || 256 * kSoftmaxRegs + 128 * kOtherRegs <= 384 * kLaunchRegs, "registers");
+  static constexpr int kSoftmaxWarps = 8 * kTiles;
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 4);      // and a warpgroup for the products and the copies (two warps idle)
+  // Two row tiles: 640 threads get 96 registers each at launch; the softmax takes 104, the others go down to 64:
+  // 512 x 104 + 128 x 64 = 640 x 96, never more than the launch got.
+  static constexpr int kLaunchRegs = 96, kSoftmaxRegs = 104, kOtherRegs = 64;
+  static_assert(kTiles == 1 || 512 * kSoftmaxRegs + 128 * kOtherRegs <= 640 * kLaunchRegs, "registers");
   static constexpr int kSmemBytes = 1024 + kTiles * kQBytes + kSlots * kSlotBytes + 256;
   static constexpr int kPieceFloats = kRows * (D + 2);
   static constexpr int kO = 256;                                 // tensor-memory column of the (first) output; S at 0 and 128
@@ -93,14 +93,22 @@ struct TileCursor {
   }
 };
 
+// The code of what seldom happens is laid out away from the loop, which is long enough to feel its instruction fetches.
+__device__ __forceinline__ bool rarely(bool x) { return __builtin_expect(x, 0); }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The largest, NaN if one is.
+__device__ __forceinline__ float max2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 // Two fp32 operations in one instruction.
@@ -117,6 +125,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
+}
+// 2^x of two values on the FMA units (x <= 8; below -126 as -126): x = n + r with n the nearest integer, 2^r by a polynomial of
+// degree 5 in r (fitted on [-1/2, 1/2] for the smallest relative error, 1 at 0: 2^-22 in fp32 arithmetic), n added to its exponent.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f), unmagic = make_float2(-12582912.f, -12582912.f), minus = make_float2(-1.f, -1.f);
+  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const float2 t = add2(x, magic);  // 1.5 2^23 + n: n in the low bits
+  const float2 r = fma2(add2(t, unmagic), minus, x);
+  float2 e = fma2(r, make_float2(1.326472731307149e-3f, 1.326472731307149e-3f), make_float2(9.671512991189957e-3f, 9.671512991189957e-3f));
+  e = fma2(e, r, make_float2(5.550733581185341e-2f, 5.550733581185341e-2f));
+  e = fma2(e, r, make_float2(0.24022242426872253f, 0.24022242426872253f));
+  e = fma2(e, r, make_float2(0.6931470036506653f, 0.6931470036506653f));
+  e = fma2(e, r, make_float2(1.f, 1.f));
+  return make_float2(__int_as_float((__float_as_int(t.x) << 23) + __float_as_int(e.x)), __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(e.y)));
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -175,15 +197,17 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t ring = base + NT * C::kQBytes;
-  __shared__ uint64_t bars[2 * C::kSlots + 9];
+  __shared__ uint64_t bars[2 * C::kSlots + 11];
   __shared__ volatile uint32_t abort_flag;
   __shared__ uint32_t tmem_word;
-  __shared__ int64_t sums[12];
+  __shared__ int64_t sums[20];
+  // What the two threads of a row tell one another: maxima (by turns: a thread may be a tile ahead), sums.
+  __shared__ float half_m[2][2][NT][128], half_l[2][NT][128];
   __shared__ int64_t start_off;
   __shared__ int start_b, start_rt, start_i;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   constexpr int kWarps = C::kThreads / 32;
-  static_assert(kWarps <= 12, "sums");
+  static_assert(kWarps <= 20, "sums");
   auto full = [&](int s) { return smem_u32(bars + s); };
   auto empty = [&](int s) { return smem_u32(bars + C::kSlots + s); };
   auto s_full = [&](int t) { return smem_u32(bars + 2 * C::kSlots + t); };
@@ -191,12 +215,13 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   auto q_ready = [&](int t) { return smem_u32(bars + 2 * C::kSlots + 4 + t); };
   auto pv_done = [&](int t) { return smem_u32(bars + 2 * C::kSlots + 6 + t); };
   const uint32_t drained = smem_u32(bars + 2 * C::kSlots + 8);
+  auto turn = [&](int t) { return smem_u32(bars + 2 * C::kSlots + 9 + t); };
 
   if (tid == 0) {
     abort_flag = 0, start_b = -1;
-    for (int s = 0; s < C::kSlots; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
-    for (int t = 0; t < 2; t++) mbar_init(s_full(t), 1), mbar_init(p_ready(t), 4), mbar_init(q_ready(t), 128), mbar_init(pv_done(t), 1);
-    mbar_init(drained, 1);
+    for (int s = 0; s < C::kSlots; s++) mbar_init(full(s), 1), mbar_init(empty(s), NT);
+    for (int t = 0; t < 2; t++) mbar_init(s_full(t), 1), mbar_init(p_ready(t), 8), mbar_init(q_ready(t), 8), mbar_init(pv_done(t), 1);
+    mbar_init(drained, NT), mbar_init(turn(0), 1), mbar_init(turn(1), 1);
     mbar_init_fence();
     prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
   }
@@ -294,24 +319,33 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
 
   if (warp >= C::kSoftmaxWarps) {
   if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-  // (two row tiles: two more warps, idle, complete the warpgroup)
-  if (warp == C::kSoftmaxWarps + 1) {
+  // (the other warps are idle: they complete the warpgroup)
+  if (warp == C::kSoftmaxWarps + NT) {
     // ---- copies -----------------------------------------------------------------------------------------------------------
     const int boxes = C::kKeys / box;  // per tile: at most eight, one per lane
     int slot = 0, issued = 0;
     uint32_t phase = 0;
     bool stop = false;  // a wait ran out (the same in all lanes)
-    auto load = [&](const CUtensorMap* map, bool values, int i) {  // all lanes
+    // Lane x looks after box x of a tile: where it lies, and whether a row sees any of its page (others are not read).
+    struct Box {
+      int tile0, k0, page;
+      bool need;
+    };
+    auto look_up = [&](int i) {
+      Box x;
+      x.tile0 = tile_of(i, cur.r.sink_tiles, cur.r.first_window_tile) * C::kKeys;
+      x.k0 = x.tile0 + lane * box, x.page = 0;
+      const int k1 = min(x.k0 + box, cur.r.reach);
+      x.need = lane < boxes && x.k0 < cur.r.reach && (x.k0 < p.sinks || k1 > cur.r.low);
+      if (x.need) x.page = p.table[cur.b * p.table_ld + x.k0 / p.page_size];
+      return x;
+    };
+    auto load = [&](const CUtensorMap* map, bool values, const Box& x) {  // all lanes
       if (stop) return;
-      const int tile0 = tile_of(i, cur.r.sink_tiles, cur.r.first_window_tile) * C::kKeys;
-      const int k0 = tile0 + lane * box, k1 = min(k0 + box, cur.r.reach);
-      const bool need = lane < boxes && k0 < cur.r.reach && (k0 < p.sinks || k1 > cur.r.low);  // pages that no row sees are not read
-      int page = 0;
-      if (need) {
-        page = p.table[cur.b * p.table_ld + k0 / p.page_size];
-        if (page < 0 || page >= p.pages) page = p.pages, atomicCAS(status, 0u, uint32_t(kStatusBadPage));  // (reads zeros)
-      }
-      const uint32_t needs = __ballot_sync(0xffffffffu, need);
+      const int tile0 = x.tile0, k0 = x.k0;
+      int page = x.page;
+      if (x.need && (page < 0 || page >= p.pages)) page = p.pages, atomicCAS(status, 0u, uint32_t(kStatusBadPage));  // (reads zeros)
+      const uint32_t needs = __ballot_sync(0xffffffffu, x.need);
 #pragma unroll
       for (int part = 0; part < C::kParts; part++) {
         // K is split along its channels, V along its keys
@@ -337,11 +371,15 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       for (; cur.any(p, t1) && !stop; cur.template next<C::kRows, C::kSegmentCost>(p, min_rows)) {
         const int from = cur.from, end = cur.end(t1);
         if (cur.s.len > cur.s.reach && lane == 0) atomicCAS(status, 0u, uint32_t(kStatusBadPage));
-        load(&kmap, false, from);
-        for (int i = from; i < end; i++) {  // the order in which the products use them
-          if (NT == 1 && i + 1 < end) load(&kmap, false, i + 1);
-          load(&vmap, true, i);
-          if (NT == 2 && i + 1 < end) load(&kmap, false, i + 1);
+        // In the order in which the products use them. The table is read a tile ahead: its latency would add to the copy's.
+        Box x = look_up(from);
+        load(&kmap, false, x);
+        for (int i = from; i < end; i++) {
+          const Box next = i + 1 < end ? look_up(i + 1) : x;
+          if (NT == 1 && i + 1 < end) load(&kmap, false, next);
+          load(&vmap, true, x);
+          if (NT == 2 && i + 1 < end) load(&kmap, false, next);
+          x = next;
         }
       }
     if (stop)  // unwinding: no copy may still be in flight when the CTA ends
@@ -350,7 +388,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
         uint32_t unused = 0;
         if (lane == 0) mbar_wait_bounded(full(s), uint32_t(last / C::kSlots) & 1u, &abort_flag, &unused, kStatusDrainTimeout);
       }
-  } else if (warp == C::kSoftmaxWarps) {
+  } else if (warp < C::kSoftmaxWarps + NT) {
     // ---- products -----------------------------------------------------------------------------------------------------------
     // The whole warp walks the segments and waits, so that addresses and descriptors stay uniform; one elected lane issues. (A
     // single-lane branch spent 115 cycles per product on moving descriptors, more than the products take.)
@@ -359,13 +397,12 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       constexpr int kPartKeys = C::kKeys / C::kParts;
       const uint64_t q_desc = umma_desc_k_sw128(base), k_desc = umma_desc_k_sw128(ring), v_desc = umma_desc_mn_sw128(ring, kPartKeys * 128);
       int slot = 0;
-      uint32_t phase = 0, p_phase = 0, q_phase = 0;  // (bit t: of row tile or S buffer t)
+      uint32_t phase = 0, p_phase = 0, q_phase = 0, turn_phase = 0;
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) {
         ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(bar, parity, &abort_flag, status, code));
         tc_fence_after_sync();
       };
-      auto wait_p = [&](int t) { wait(p_ready(t), (p_phase >> t) & 1u, kStatusAccumWaitTimeout), p_phase ^= 1u << t; };
       auto advance = [&] { if (++slot == C::kSlots) slot = 0, phase ^= 1u; };
       // S of row tile t into buffer `buf` from the K part in ring slot s
       auto qk_part = [&](int t, int buf, int s, int part) {
@@ -379,60 +416,57 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       };
       auto pv_part = [&](int t, int buf, int s, int part, bool accumulate) {
         const uint64_t vd = v_desc + uint64_t(s * (C::kSlotBytes >> 4));
-        const uint32_t d = tmem + C::kO + t * D, a = tmem + buf * 128 + part * (kPartKeys / 2);
+        const uint32_t d = tmem + C::kO + t * D, a = tmem + buf * 128 + part * 64;
 #pragma unroll
-        for (int k = 0; k < kPartKeys / 16; k++) umma_f16_ts(d, a + k * 8, vd + ((k * 2048) >> 4), pv_idesc, k > 0 || accumulate);
+        for (int k = 0; k < kPartKeys / 16; k++) umma_f16_ts(d, a + (k / 4) * 64 + (k % 4) * 8, vd + ((k * 2048) >> 4), pv_idesc, k > 0 || accumulate);
       };
+      const int mine = warp - C::kSoftmaxWarps;
       for (; cur.any(p, t1) && ok; cur.template next<C::kRows, C::kSegmentCost>(p, min_rows)) {
         const int from = cur.from, end = cur.end(t1);
-        const int active = min(C::kRows, cur.rows - cur.rt * C::kRows) > 128 ? 2 : 1;
-        for (int x = 0; x < active; x++) wait(q_ready(x), (q_phase >> x) & 1u, kStatusAccumWaitTimeout), q_phase ^= 1u << x;
         if constexpr (NT == 2) {
-          wait(full(slot), phase, kStatusFullWaitTimeout);
-          if (!ok) break;
-          if (elect_one()) {
-            for (int x = 0; x < active; x++) qk_part(x, x, slot, 0), umma_commit(s_full(x));
-            umma_commit(empty(slot));
-          }
-          __syncwarp();
-          advance();
-          for (int i = from; i < end; i++) {
-            const bool more = i + 1 < end;
-            const int vs = slot;
-            wait(full(slot), phase, kStatusFullWaitTimeout);  // V of this tile
-            advance();
-            wait_p(0);
-            if (more) wait(full(slot), phase, kStatusFullWaitTimeout);  // K of the next
+          // A warp per row tile: while one waits, the other's products keep the tensor cores busy. They issue in turns: products of
+          // both tiles mixed together would end together, and so would the softmaxes between them. A tile without rows in this segment
+          // only gives the ring slots back.
+          const bool both = cur.rows - cur.rt * C::kRows > 128;
+          auto my_turn = [&] {
+            if (both) wait(turn(mine), turn_phase ^ uint32_t(mine == 0), kStatusAccumWaitTimeout), turn_phase ^= 1u;
+          };
+          auto pass_turn = [&] {
+            if (both) mbar_arrive(turn(mine ^ 1));
+          };
+          if (both || mine == 0) {
+            wait(q_ready(mine), q_phase, kStatusAccumWaitTimeout), q_phase ^= 1u;
+            wait(full(slot), phase, kStatusFullWaitTimeout);
+            my_turn();
             if (!ok) break;
-            if (elect_one()) {
-              pv_part(0, 0, vs, 0, i > from);
-              if (active == 1) umma_commit(empty(vs));
-              if (more) {
-                qk_part(0, 0, slot, 0);
-                umma_commit(s_full(0));
-                if (active == 1) umma_commit(empty(slot));
-              } else {
-                umma_commit(pv_done(0));
-              }
-            }
+            if (elect_one()) qk_part(mine, mine, slot, 0), umma_commit(s_full(mine)), pass_turn(), umma_commit(empty(slot));
             __syncwarp();
-            if (active == 2) {
-              wait_p(1);
+            advance();
+            for (int i = from; i < end; i++) {
+              const int vs = slot;
+              wait(full(slot), phase, kStatusFullWaitTimeout);  // V of this tile
+              advance();
+              const bool more = i + 1 < end;
+              if (more) wait(full(slot), phase, kStatusFullWaitTimeout);  // K of the next
+              wait(p_ready(mine), p_phase, kStatusAccumWaitTimeout), p_phase ^= 1u;
+              my_turn();
               if (!ok) break;
               if (elect_one()) {
-                pv_part(1, 1, vs, 0, i > from);
-                umma_commit(empty(vs));
-                if (more) {
-                  qk_part(1, 1, slot, 0);
-                  umma_commit(s_full(1));
-                  umma_commit(empty(slot));
-                } else {
-                  umma_commit(pv_done(1));
-                }
+                pv_part(mine, mine, vs, 0, i > from);
+                if (more)
+                  qk_part(mine, mine, slot, 0), umma_commit(s_full(mine)), pass_turn(), umma_commit(empty(vs)), umma_commit(empty(slot));
+                else
+                  umma_commit(pv_done(mine)), pass_turn(), umma_commit(empty(vs));
               }
               __syncwarp();
+              if (more) advance();
             }
-            if (more) advance();
+          } else {
+            for (int i = 0; i < 2 * (end - from) && ok; i++) {
+              wait(full(slot), phase, kStatusFullWaitTimeout);
+              if (lane == 0) mbar_arrive(empty(slot));
+              advance();
+            }
           }
         } else {
           auto qk = [&](int buf) {
@@ -447,11 +481,12 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
               advance();
             }
           };
+          wait(q_ready(0), q_phase, kStatusAccumWaitTimeout), q_phase ^= 1u;
           int buf = 0;  // of the tile whose P comes next; every segment starts at 0
           qk(0);
           for (int i = from; i < end && ok; i++) {
             if (i + 1 < end) qk(buf ^ 1);
-            wait_p(buf);
+            wait(p_ready(buf), (p_phase >> buf) & 1u, kStatusAccumWaitTimeout), p_phase ^= 1u << buf;  // (bit b: of S buffer b)
             for (int part = 0; part < C::kParts && ok; part++) {
               wait(full(slot), phase, kStatusFullWaitTimeout);
               if (ok && elect_one()) {
@@ -475,27 +510,30 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   }
   } else {
     if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
-    // ---- softmax, scaling, epilogue: one thread per row ---------------------------------------------------------------------
-    const int tile = warp / 4, row_in_tile = tid % 128;
-    const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16;
+    // ---- softmax, scaling, epilogue: two threads per row, each with half the keys of S and half the channels of O ------------------
+    const int tile = warp / 8, half = (warp / 4) % 2, row_in_tile = (warp % 4) * 32 + lane;
+    const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16, o_at = tmem + lanes + C::kO + tile * D + half * (D / 2);
     const float c2 = fabsf(p.scale) * 1.4426950408889634f, scale_log2 = c2 > 0.f ? c2 : 1e-30f;  // (0 would turn a masked -infinity into NaN)
     const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale goes into the queries' signs
-    uint32_t s_phase[2] = {0, 0}, pv_phase = 0;
+    auto pair_bar = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + warp % 4) : "memory"); };  // the two warps of 32 rows
+    uint32_t s_phase = 0, pv_phase = 0;  // (bit b: of S buffer b)
     int chunk = 0;  // ring places used before this segment
-    // this thread's row of the segment at `at` into shared memory, in the layout of the products' operands
+    // this thread's half of its row of the segment at `at` into shared memory, in the layout of the products' operands
     auto load_q = [&](const TileCursor& at) {
       const int row = at.rt * C::kRows + tile * 128 + row_in_tile;
       const uint16_t* src = static_cast<const uint16_t*>(p.q) + (at.s.row0 + row / G) * p.q_ld_token + (at.hk * G + row % G) * p.q_ld_head;
       const uint32_t dst = base + tile * C::kQBytes + row_in_tile * 128;
       const bool live = row < at.rows;
 #pragma unroll
-      for (int d = 0; d < D / 8; d++) {
+      for (int x = 0; x < D / 16; x++) {
+        const int d = half * (D / 16) + x;
         uint4 v = live ? reinterpret_cast<const uint4*>(src)[d] : make_uint4(0, 0, 0, 0);
         v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (d / 8) * 128 * 128 + (((d % 8) ^ (row_in_tile & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
       }
       fence_proxy_async_smem();
-      mbar_arrive(q_ready(tile));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready(tile));
     };
     auto in_use = [&](const TileCursor& at) { return at.rows - at.rt * C::kRows > tile * 128; };
     if (work && cur.any(p, t1) && in_use(cur)) load_q(cur);
@@ -508,70 +546,85 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       if (in_use(cur)) {
         const int row = cur.rt * C::kRows + tile * 128 + row_in_tile, row_end = min(cur.rows, cur.rt * C::kRows + tile * 128 + 128);
         const int first = cur.s.len - cur.s.rows, pos = first + row / G;
-        const int tile_pmin = first + (cur.rt * C::kRows + tile * 128) / G, tile_pmax = first + (row_end - 1) / G;
         const bool warp_live = cur.rt * C::kRows + tile * 128 + (warp % 4) * 32 < cur.rows;  // a warp without rows only keeps step
-        float m = -INFINITY, l = 0.f;
+        // Tiles that start in [whole_lo, whole_hi) or before whole_sinks are seen in full by every row of this row tile; those in
+        // [held_lo, held_hi) or before held_sinks hold no key that no row of the segment sees.
+        const int pmin = first + (cur.rt * C::kRows + tile * 128) / G, pmax = first + (row_end - 1) / G;
+        const int whole_hi = min(pmin + 1, cur.r.reach) - C::kKeys + 1, whole_lo = p.window > 0 ? pmax - p.window + 1 : 0;
+        const int held_hi = cur.r.reach - C::kKeys + 1, held_lo = cur.r.low, sinks_hi = p.sinks - C::kKeys + 1;
+        float m = -INFINITY, l = 0.f, mc = 0.f;  // mc: what is taken off the scaled scores
         for (int i = from; i < end; i++) {
           const int buf = NT == 2 ? tile : (i - from) & 1;
-          const uint32_t s_at = tmem + lanes + buf * 128;
-          const int k0 = tile_of(i, cur.r.sink_tiles, cur.r.first_window_tile) * C::kKeys, k1 = k0 + C::kKeys - 1;
-          const bool here = !abort_flag && mbar_wait_bounded(s_full(buf), s_phase[buf], &abort_flag, status, kStatusAccumWaitTimeout);
-          s_phase[buf] ^= 1u;
-          if (!__all_sync(0xffffffffu, here)) continue;
+          const uint32_t s_at = tmem + lanes + buf * 128 + half * 64;
+          const int k0 = tile_of(i, cur.r.sink_tiles, cur.r.first_window_tile) * C::kKeys;
+          const bool edge = !(k0 < whole_hi && (k0 >= whole_lo || k0 < sinks_hi));
+          const bool here = mbar_wait_bounded(s_full(buf), (s_phase >> buf) & 1u, &abort_flag, status, kStatusAccumWaitTimeout);
+          s_phase ^= 1u << buf;
           tc_fence_after_sync();
           auto wait_pv = [&] {  // of the tile before (kTiles == 1): it may still be adding to O
             mbar_wait_bounded(pv_done(0), pv_phase ^ 1u, &abort_flag, status, kStatusAccumWaitTimeout);
             tc_fence_after_sync();
           };
           if (warp_live) {
-            float s[128];
+            // The maximum needs all 64 scores, the exponentials 32 at a time: they are read from tensor memory twice instead of being held.
+            float tile_m;
+            {
+              float s[64];
+              tmem_ld32(s_at, s), tmem_ld32(s_at + 32, s + 32);
+              tmem_ld_wait();
+              if (rarely(edge)) {
+                const int at = k0 + half * 64, hi = min(pos, cur.r.reach - 1) - at, lo = p.window > 0 ? pos - p.window + 1 - at : -1, si = p.sinks - at;
 #pragma unroll
-            for (int x = 0; x < 4; x++) tmem_ld32(s_at + 32 * x, s + 32 * x);
-            tmem_ld_wait();
-            const bool all = k1 <= tile_pmin && k1 < cur.r.reach && (p.window == 0 || k0 > tile_pmax - p.window || k1 < p.sinks);
-            if (!all) {
-              const int hi = min(pos, cur.r.reach - 1) - k0, lo = p.window > 0 ? pos - p.window + 1 - k0 : -1, si = p.sinks - k0;
+                for (int x = 0; x < 64; x++) s[x] = x <= hi && (x >= lo || x < si) ? s[x] : -INFINITY;
+                tmem_st32(s_at, reinterpret_cast<uint32_t*>(s)), tmem_st32(s_at + 32, reinterpret_cast<uint32_t*>(s + 32));
+                tmem_st_wait();
+              }
+              float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-              for (int x = 0; x < 128; x++) s[x] = x <= hi && (x >= lo || x < si) ? s[x] : -INFINITY;
+              for (int x = 4; x < 60; x += 2) top[(x / 2) & 3] = max3(top[(x / 2) & 3], s[x], s[x + 1]);
+              top[0] = max3(top[0], s[60], s[61]), top[1] = max3(top[1], s[62], s[63]);
+              tile_m = max2(max3(top[0], top[1], top[2]), top[3]);
             }
-            float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int x = 4; x < 124; x += 2) top[(x / 2) & 3] = max3(top[(x / 2) & 3], s[x], s[x + 1]);
-            top[0] = max3(top[0], s[124], s[125]), top[1] = max3(top[1], s[126], s[127]);
-            const float tile_m = fmaxf(max3(top[0], top[1], top[2]), top[3]);
-            const bool grow = m == -INFINITY ? tile_m > m : (tile_m - m) * scale_log2 > 8.f;
-            if (__any_sync(0xffffffffu, grow)) {
+            half_m[(i - from) & 1][half][tile][row_in_tile] = tile_m;
+            pair_bar();
+            tile_m = max2(tile_m, half_m[(i - from) & 1][half ^ 1][tile][row_in_tile]);
+            // (m = -infinity: everything that is seen grows; a NaN is taken over and makes the row NaN)
+            const bool grow = !((tile_m - m) * scale_log2 <= 8.f) && tile_m != -INFINITY;
+            if (rarely(__any_sync(0xffffffffu, grow))) {
               const float f = grow ? exp2_fast((m - tile_m) * scale_log2) : 1.f;  // (m = -infinity: 0)
-              if (grow) m = tile_m, l *= f;
+              if (grow) m = tile_m, mc = m * scale_log2, l *= f;
               if (i > from) {
                 if (NT == 1) wait_pv();
 #pragma unroll
-                for (int d = 0; d < D; d += 32) {
+                for (int d = 0; d < D / 2; d += 32) {
                   float o[32];
-                  tmem_ld32(tmem + lanes + C::kO + tile * D + d, o);
+                  tmem_ld32(o_at + d, o);
                   tmem_ld_wait();
 #pragma unroll
                   for (int x = 0; x < 32; x++) o[x] *= f;
-                  tmem_st32(tmem + lanes + C::kO + tile * D + d, reinterpret_cast<uint32_t*>(o));
+                  tmem_st32(o_at + d, reinterpret_cast<uint32_t*>(o));
                 }
               }
             }
-            const float mc = m == -INFINITY ? 0.f : m * scale_log2;
             const float2 scale2 = make_float2(scale_log2, scale_log2), off2 = make_float2(-mc, -mc);
             float2 sum[2] = {};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-              uint32_t w[32];
+              float s[32];
+              uint32_t w[16];
+              tmem_ld32(s_at + 32 * h, s);
+              tmem_ld_wait();
 #pragma unroll
-              for (int x = 0; x < 32; x++) {
-                float2 e = fma2(make_float2(s[64 * h + 2 * x], s[64 * h + 2 * x + 1]), scale2, off2);
-                e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+              for (int x = 0; x < 16; x++) {
+                float2 e = fma2(make_float2(s[2 * x], s[2 * x + 1]), scale2, off2);
+                // the special-function units alone would need as long as the products: some of the pairs go through the FMA units
+                e = x % C::kPolyEvery == 1 ? exp2_poly(e) : make_float2(exp2_fast(e.x), exp2_fast(e.y));
                 sum[x & 1] = add2(sum[x & 1], e);
                 T2 v;
                 narrow(e, &v);
                 w[x] = *reinterpret_cast<uint32_t*>(&v);
               }
-              tmem_st32(s_at + 32 * h, w);
+              tmem_st16(s_at + 16 * h, reinterpret_cast<const uint4(&)[4]>(w));  // (over scores that have been read)
             }
             sum[0] = add2(sum[0], sum[1]);
             l += sum[0].x + sum[0].y;
@@ -584,21 +637,21 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
             pv_phase ^= 1u;
           }
           // Values of keys that no row of the segment sees are whatever the cache (or an earlier tile) left there, and 0 x NaN would be
-          // NaN: the first warpgroup, whose P every product waits for, clears them.
-          if (tile == 0 && !(k1 <= cur.r.pmin && k1 < cur.r.reach && (p.window == 0 || k0 > cur.r.pmin - p.window || k1 < p.sinks))) {
+          // NaN: each row tile clears them before its own product, two threads to a key.
+          if (rarely(edge && here && !(k0 < held_hi && (k0 >= held_lo || k0 < sinks_hi)))) {
             const int key = k0 + row_in_tile;
-            const bool any = key < cur.r.reach && (p.window == 0 || key > cur.r.pmin - p.window || key < p.sinks);
+            const bool any = key < cur.r.reach && (key >= held_lo || key < p.sinks);
             const int n = end - from, j = i - from;
             int at = chunk + (NT == 2 ? 2 * j + 1 : C::kParts * min(2 * j + 2, 2 * n - 1));  // ring place of this V tile
             constexpr int kPartKeys = C::kKeys / C::kParts;
             at += row_in_tile / kPartKeys;
             if (!any) {
               mbar_wait_bounded(full(at % C::kSlots), uint32_t(at / C::kSlots) & 1u, &abort_flag, status, kStatusFullWaitTimeout);
-              const uint32_t dst = ring + (at % C::kSlots) * C::kSlotBytes + (row_in_tile % kPartKeys) * 128;
+              const uint32_t dst = ring + (at % C::kSlots) * C::kSlotBytes + (row_in_tile % kPartKeys) * 128 + half * 64;
 #pragma unroll
               for (int d = 0; d < D / 64; d++)
 #pragma unroll
-                for (int x = 0; x < 8; x++)
+                for (int x = 0; x < 4; x++)
                   asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst + d * kPartKeys * 128 + x * 16), "r"(0) : "memory");
               fence_proxy_async_smem();
             }
@@ -610,37 +663,43 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
         // every product with this segment's Q has ended (its S was read): the next segment's may take its place
         load_next_q(cur);
         // the last product of the segment, then its result
-        const bool done = !abort_flag && mbar_wait_bounded(pv_done(tile), NT == 2 ? pv_phase : pv_phase ^ 1u, &abort_flag, status, kStatusAccumWaitTimeout);
+        const bool done = mbar_wait_bounded(pv_done(tile), NT == 2 ? pv_phase : pv_phase ^ 1u, &abort_flag, status, kStatusAccumWaitTimeout);
         if (NT == 2) pv_phase ^= 1u;
-        if (__all_sync(0xffffffffu, done) && warp_live) {
+        if (warp_live) {
           tc_fence_after_sync();
-          const bool whole = from == 0 && end == cur.r.tiles, live = row < cur.rows;
+          half_l[half][tile][row_in_tile] = l;
+          pair_bar();
+          l += half_l[half ^ 1][tile][row_in_tile];
+          if (m == -INFINITY) l = 0.f;  // (a row that sees nothing: its 2^-126s are not sums)
+          const bool whole = from == 0 && end == cur.r.tiles, live = row < cur.rows && done;
           const float inv = l == 0.f ? 0.f : 1.f / l;
-          uint16_t* out = static_cast<uint16_t*>(p.out) + (cur.s.row0 + row / G) * p.out_ld_token + (cur.hk * G + row % G) * p.out_ld_head;
+          uint16_t* out = static_cast<uint16_t*>(p.out) + (cur.s.row0 + row / G) * p.out_ld_token + (cur.hk * G + row % G) * p.out_ld_head + half * (D / 2);
           float* piece = pieces + (2 * c + (from > 0 ? 0 : 1)) * C::kPieceFloats;
 #pragma unroll
-          for (int d = 0; d < D; d += 32) {
+          for (int d = 0; d < D / 2; d += 32) {
             float o[32];
-            tmem_ld32(tmem + lanes + C::kO + tile * D + d, o);
+            tmem_ld32(o_at + d, o);
             tmem_ld_wait();
             if (whole && live) {
 #pragma unroll
               for (int x = 0; x < 32; x += 8) {
                 T2 w[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) narrow(make_float2(o[x + 2 * e] * inv, o[x + 2 * e + 1] * inv), &w[e]);
+                for (int e = 0; e < 4; e++) narrow(l == 0.f ? make_float2(0.f, 0.f) : make_float2(o[x + 2 * e] * inv, o[x + 2 * e + 1] * inv), &w[e]);
                 *reinterpret_cast<uint4*>(out + d + x) = *reinterpret_cast<uint4*>(w);
               }
             }
             if (!whole && live) {  // channel groups of four, rows side by side: a warp's stores are contiguous
 #pragma unroll
               for (int x = 0; x < 32; x += 4)
-                *reinterpret_cast<float4*>(piece + ((d + x) / 4 * C::kRows + tile * 128 + row_in_tile) * 4) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+                *reinterpret_cast<float4*>(piece + ((half * (D / 2) + d + x) / 4 * C::kRows + tile * 128 + row_in_tile) * 4) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
             }
           }
-          const float mb = m * scale_log2;  // (-infinity stays)
-          if (whole && live && p.lse) p.lse[int64_t(cur.s.row0 + row / G) * p.heads + cur.hk * G + row % G] = l == 0.f ? -INFINITY : (mb + log2f(l)) * 0.6931471805599453f;
-          if (!whole && live) piece[C::kRows * D + tile * 128 + row_in_tile] = mb, piece[C::kRows * (D + 1) + tile * 128 + row_in_tile] = l;
+          if (half == 0) {
+            const float mb = m * scale_log2;  // (-infinity stays)
+            if (whole && live && p.lse) p.lse[int64_t(cur.s.row0 + row / G) * p.heads + cur.hk * G + row % G] = l == 0.f ? -INFINITY : (mb + log2f(l)) * 0.6931471805599453f;
+            if (!whole && live) piece[C::kRows * D + tile * 128 + row_in_tile] = mb, piece[C::kRows * (D + 1) + tile * 128 + row_in_tile] = l;
+          }
           tc_fence_before_sync();
         }
       } else {
@@ -675,7 +734,8 @@ __global__ void __launch_bounds__(128) attention_tile_join_kernel(const __grid_c
   float4 o[8] = {};
   for (int i = 0; i < r.pieces; i++) {
     const float* x = piece(i);
-    const float mi = x[C::kRows * D + in_seg], f = mi == -INFINITY ? 0.f : exp2_fast(mi - m);
+    const float mi = x[C::kRows * D + in_seg], f = exp2_fast(mi - m);
+    if (mi == -INFINITY) continue;
     l += f * x[C::kRows * (D + 1) + in_seg];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
