@@ -17,7 +17,10 @@
 //
 // Programmatic dependent launch: as every kernel of this library, wait for the predecessor first, release the successor
 // only then.
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
+
 #include <cuda_fp16.h>
 
 #include "../../include/q27b200/capi.h"
@@ -29,32 +32,58 @@ namespace {
 
 using Args = q27b_qk_rope;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kMostTokens = 4;
 
-// Four consecutive channels.
-__device__ __forceinline__ void load4(const float* p, float* v) {
-  const float4 t = *reinterpret_cast<const float4*>(p);
-  v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-}
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float* v) {
-  const uint2 t = *reinterpret_cast<const uint2*>(p);
-  v[0] = __uint_as_float(t.x << 16), v[1] = __uint_as_float(t.x & 0xFFFF0000u);
-  v[2] = __uint_as_float(t.y << 16), v[3] = __uint_as_float(t.y & 0xFFFF0000u);
-}
-__device__ __forceinline__ void load4(const __half* p, float* v) {
-  const uint2 t = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&t.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&t.y));
-  v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-}
+// kUnit consecutive channels as they lie in memory, and widened.
+template <typename E, int kUnit>
+struct Raw {
+  static constexpr int kBytes = kUnit * int(sizeof(E)), kVectors = kBytes > 16 ? kBytes / 16 : 1;
+  uint4 v[kVectors];  // (8 bytes: the lower half)
+  __device__ __forceinline__ void load(const E* p) {
+    if constexpr (kBytes == 8) {
+      const uint2 t = *reinterpret_cast<const uint2*>(p);
+      v[0].x = t.x, v[0].y = t.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVectors; i++) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+  }
+  __device__ __forceinline__ void widen(float* x) const {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+#pragma unroll
+    for (int i = 0; i < kUnit; i++) {
+      if constexpr (sizeof(E) == 4)
+        x[i] = __uint_as_float(w[i]);
+      else if constexpr (std::is_same<E, __nv_bfloat16>::value)
+        x[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+      else
+        x[i] = __half2float(__ushort_as_half(uint16_t(i % 2 ? w[i / 2] >> 16 : w[i / 2])));
+    }
+  }
+};
 // The one rounding of a result to its type (nearest even).
-__device__ __forceinline__ void store4(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* v) {
-  __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
-  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+template <int kUnit>
+__device__ __forceinline__ void store(float* p, const float* v) {
+#pragma unroll
+  for (int i = 0; i < kUnit; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
 }
-__device__ __forceinline__ void store4(__half* p, const float* v) {
-  __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
+template <int kUnit, typename Out>
+__device__ __forceinline__ void store(Out* p, const float* v) {
+  uint32_t w[kUnit / 2];
+#pragma unroll
+  for (int i = 0; i < kUnit / 2; i++) {
+    if constexpr (std::is_same<Out, __nv_bfloat16>::value) {
+      __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<uint32_t*>(&t);
+    } else {
+      __half2 t = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<uint32_t*>(&t);
+    }
+  }
+  if constexpr (kUnit == 8)
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else
+    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 
 // cos and sin of a binary fraction of a turn, times the amplitude.
@@ -69,146 +98,161 @@ __device__ __forceinline__ float2 cos_sin_turn(uint64_t turn, float amplitude) {
   return make_float2(c1 * sign, s1 * sign);
 }
 
-template <typename W>
-__device__ __forceinline__ void load_weight(const W* w, int at, bool zero_centred, float* v) {
-  load4(w + at, v);
-#pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = zero_centred ? 1.f + v[i] : v[i];
+__device__ __forceinline__ void turn_pair(float& a, float& b, float2 cs) {
+  const float u = a * cs.x - b * cs.y;
+  b = a * cs.y + b * cs.x, a = u;
 }
 
-template <typename In, typename Out, int kLanes>
+// kLanes lanes to a row, kUnit * 2 channels (kUnit pairs, or two runs that do not turn) to a lane; `tokens` tokens to a CTA.
+template <typename In, typename Out, int kUnit, int kLanes>
 __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant__ Args p, int tokens, uint32_t* status) {
-  extern __shared__ float2 table[];  // [tokens of this CTA][rot / 2] (cos, sin)
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int D = p.head_dim, pairs = p.rot_dim / 2, t0 = blockIdx.x * tokens, nt = min(tokens, p.T - t0);
+  float2* table = reinterpret_cast<float2*>(smem);                   // [tokens][pairs] (cos, sin)
+  float* weights = reinterpret_cast<float*>(table + tokens * pairs);  // [2][D] what q and k are multiplied by (with the norm)
+  __shared__ int64_t place_of[kMostTokens];
+  const bool norm = p.q_weight != nullptr;
   pdl_wait();
   pdl_trigger();
-  const int t0 = blockIdx.x * tokens, nt = min(tokens, p.T - t0), pairs = p.rot_dim / 2;
   for (int i = threadIdx.x; i < nt * pairs; i += kThreads) {
     const int t = t0 + i / pairs;
     const int64_t pos = p.pos64 ? static_cast<const int64_t*>(p.positions)[t] : int64_t(static_cast<const int32_t*>(p.positions)[t]);
     table[i] = cos_sin_turn(uint64_t(pos) * p.turns[i % pairs], p.amplitude);
   }
-  const int lane = threadIdx.x % kLanes, D = p.head_dim;
-  const bool active = lane * 8 < D, turns = lane * 8 < p.rot_dim;
-  int a, b;  // the two groups of four channels of this lane
-  if (p.interleaved || !turns)
-    a = lane * 8, b = a + 4;
-  else
-    a = lane * 4, b = pairs + lane * 4;
-  float wq[8], wk[8];
-  const bool norm = p.q_weight != nullptr;
-  if (norm && active) {
-    if (p.weight_f32) {
-      load_weight(static_cast<const float*>(p.q_weight), a, p.zero_centred, wq), load_weight(static_cast<const float*>(p.q_weight), b, p.zero_centred, wq + 4);
-      load_weight(static_cast<const float*>(p.k_weight), a, p.zero_centred, wk), load_weight(static_cast<const float*>(p.k_weight), b, p.zero_centred, wk + 4);
-    } else {
-      using B = __nv_bfloat16;
-      load_weight(static_cast<const B*>(p.q_weight), a, p.zero_centred, wq), load_weight(static_cast<const B*>(p.q_weight), b, p.zero_centred, wq + 4);
-      load_weight(static_cast<const B*>(p.k_weight), a, p.zero_centred, wk), load_weight(static_cast<const B*>(p.k_weight), b, p.zero_centred, wk + 4);
+  if (norm)
+    for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
+      const void* w = i < D ? p.q_weight : p.k_weight;
+      const int d = i < D ? i : i - D;
+      const float v = p.weight_f32 ? static_cast<const float*>(w)[d] : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[d]);
+      weights[i] = p.zero_centred ? 1.f + v : v;
     }
+  if (p.slots && threadIdx.x < nt) {  // the tokens' places in the cache: page and offset, -1: not written
+    const int64_t slot = p.slots[t0 + threadIdx.x], page = slot < 0 ? -1 : slot / p.page_size;
+    if (page >= p.pages) atomicCAS(status, 0u, uint32_t(kStatusBadSlot));
+    place_of[threadIdx.x] = page < 0 || page >= p.pages ? -1 : (page << 32) | (slot - page * p.page_size);
   }
   __syncthreads();
 
-  const int vheads = p.v ? p.k_heads : 0, rows = p.q_heads + p.k_heads + vheads;
-  const int step = (kThreads / kLanes) * gridDim.y;
-  const float inv_dim = 1.f / float(D);  // exact or rounded once: D <= 256
-  // grid.y shares the rows of a token group out when there are few tokens
-  // (the loop runs the same number of times in every lane of a warp: the shuffles below are whole-warp)
-  const int total = nt * rows;
-  for (int r0 = blockIdx.y * (kThreads / kLanes); r0 < total; r0 += step) {
-    const int r = r0 + threadIdx.x / kLanes;
-    const bool live = active && r < total;
-    const int tl = live ? r / rows : 0, t = t0 + tl;
-    int head = live ? r - tl * rows : 0;
-    const int kind = head < p.q_heads ? 0 : head < p.q_heads + p.k_heads ? 1 : 2;
-    head -= kind == 0 ? 0 : kind == 1 ? p.q_heads : p.q_heads + p.k_heads;
-    float x[8] = {};
-    if (live) {
-      const In* src = kind == 0 ? static_cast<const In*>(p.q) + t * p.q_ld_token + head * p.q_ld_head
-                    : kind == 1 ? static_cast<const In*>(p.k) + t * p.k_ld_token + head * p.k_ld_head
-                                : static_cast<const In*>(p.v) + t * p.v_ld_token + head * p.v_ld_head;
-      load4(src + a, x), load4(src + b, x + 4);
-    }
+  // The CTA's row groups are dealt out to its tokens; a group walks the heads of its token (q, then k, then v).
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, per_token = kThreads / kLanes / tokens;
+  const int tl = group / per_token, t = t0 + tl, step = per_token * gridDim.y;
+  const int qk_heads = p.q_heads + p.k_heads, rows = qk_heads + (p.v ? p.k_heads : 0);
+  const bool active = lane * 2 * kUnit < D && tl < nt, turns = lane * 2 * kUnit < p.rot_dim;
+  int a, b;  // the two runs of kUnit channels of this lane
+  if (p.interleaved || !turns)
+    a = lane * 2 * kUnit, b = a + kUnit;
+  else
+    a = lane * kUnit, b = pairs + lane * kUnit;
+  float2 cs[kUnit];
+  if (active && turns) {
+#pragma unroll
+    for (int i = 0; i < kUnit; i++) cs[i] = table[tl * pairs + lane * kUnit + i];
+  }
+  auto source = [&](int head) {
+    return head < p.q_heads ? static_cast<const In*>(p.q) + t * p.q_ld_token + head * p.q_ld_head
+           : head < qk_heads ? static_cast<const In*>(p.k) + t * p.k_ld_token + (head - p.q_heads) * p.k_ld_head
+                             : static_cast<const In*>(p.v) + t * p.v_ld_token + (head - qk_heads) * p.v_ld_head;
+  };
+  Raw<In, kUnit> next[2];
+  int head = blockIdx.y * per_token + group % per_token;
+  if (active && head < rows) next[0].load(source(head) + a), next[1].load(source(head) + b);
+  const float inv_dim = 1.f / float(D);
+  // (the loop runs equally often in all lanes of a warp: its shuffles are whole-warp)
+  for (int h0 = blockIdx.y * per_token; h0 < rows; h0 += step, head += step) {
+    const bool live = active && head < rows;
+    float x[2 * kUnit];
+    next[0].widen(x), next[1].widen(x + kUnit);
+    if (active && head + step < rows) next[0].load(source(head + step) + a), next[1].load(source(head + step) + b);  // in flight meanwhile
     if (norm) {
       float ss = 0.f;
+      if (live) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+        for (int i = 0; i < 2 * kUnit; i++) ss = fmaf(x[i], x[i], ss);
+      }
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (kind < 2) {
+      if (live && head < qk_heads) {
         const float rms = rsqrtf(ss * inv_dim + p.eps);
+        const float* w = weights + (head < p.q_heads ? 0 : D);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] *= rms * (kind == 0 ? wq[i] : wk[i]);
+        for (int i = 0; i < kUnit; i += 4) {
+          const float4 wa = *reinterpret_cast<const float4*>(w + a + i), wb = *reinterpret_cast<const float4*>(w + b + i);
+          x[i] *= rms * wa.x, x[i + 1] *= rms * wa.y, x[i + 2] *= rms * wa.z, x[i + 3] *= rms * wa.w;
+          x[kUnit + i] *= rms * wb.x, x[kUnit + i + 1] *= rms * wb.y, x[kUnit + i + 2] *= rms * wb.z, x[kUnit + i + 3] *= rms * wb.w;
+        }
       }
     }
     if (!live) continue;
-    if (kind < 2 && turns) {
-      const float2* cs = table + tl * pairs + lane * 4;
+    if (head < qk_heads && turns) {
       if (p.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float2 e = cs[i];
-          const float u = x[2 * i], v = x[2 * i + 1];
-          x[2 * i] = u * e.x - v * e.y, x[2 * i + 1] = u * e.y + v * e.x;
-        }
+        for (int i = 0; i < kUnit; i++) turn_pair(x[2 * i], x[2 * i + 1], cs[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float2 e = cs[i];
-          const float u = x[i], v = x[i + 4];
-          x[i] = u * e.x - v * e.y, x[i + 4] = u * e.y + v * e.x;
-        }
+        for (int i = 0; i < kUnit; i++) turn_pair(x[i], x[i + kUnit], cs[i]);
       }
     }
     Out* dst;
-    if (kind == 0) {
+    if (head < p.q_heads) {
       dst = static_cast<Out*>(p.q_out) + t * p.q_out_ld_token + head * p.q_out_ld_head;
     } else if (p.slots) {
-      const int64_t slot = p.slots[t];
-      if (slot < 0) continue;  // a padding token: nothing is written
-      const int64_t page = slot / p.page_size, at = slot - page * p.page_size;
-      if (page >= p.pages) {  // no such place in the cache
-        atomicCAS(status, 0u, uint32_t(kStatusBadSlot));
-        continue;
-      }
-      dst = kind == 1 ? static_cast<Out*>(p.k_cache) + page * p.kc_ld_page + head * p.kc_ld_head + at * p.kc_ld_slot
-                      : static_cast<Out*>(p.v_cache) + page * p.vc_ld_page + head * p.vc_ld_head + at * p.vc_ld_slot;
+      const int64_t place = place_of[tl];
+      if (place < 0) continue;  // not written
+      const int64_t page = place >> 32, at = place & 0xffffffff;
+      dst = head < qk_heads ? static_cast<Out*>(p.k_cache) + page * p.kc_ld_page + (head - p.q_heads) * p.kc_ld_head + at * p.kc_ld_slot
+                            : static_cast<Out*>(p.v_cache) + page * p.vc_ld_page + (head - qk_heads) * p.vc_ld_head + at * p.vc_ld_slot;
     } else {
-      dst = static_cast<Out*>(p.k_out) + t * p.k_out_ld_token + head * p.k_out_ld_head;
+      dst = static_cast<Out*>(p.k_out) + t * p.k_out_ld_token + (head - p.q_heads) * p.k_out_ld_head;
     }
-    store4(dst + a, x), store4(dst + b, x + 4);
+    store<kUnit>(dst + a, x), store<kUnit>(dst + b, x + kUnit);
   }
 }
 
 size_t type_size(int dtype) { return dtype == Q27B_F32 ? 4 : 2; }
 
-template <typename In, typename Out, int kLanes>
+template <typename In, typename Out, int kUnit, int kLanes>
 int launch(const Args& p, cudaStream_t s) {
   const int rows = p.q_heads + p.k_heads + (p.v ? p.k_heads : 0), groups = kThreads / kLanes;
   const int sms = sm_count();
-  // Many tokens: four to a CTA, so that the cos / sin table costs one evaluation per thread. Few: one to a CTA, and its
+  // Many tokens: four to a CTA, so that the cos / sin table costs about one evaluation per thread. Few: one to a CTA, and its
   // rows shared out over grid.y until the CTAs fill the GPU.
-  const int tokens = p.T >= 4 * 8 * sms ? 4 : 1;
+  const int tokens = p.T >= 4 * 4 * sms ? kMostTokens : 1;
   const int blocks = (p.T + tokens - 1) / tokens;
   int share = 1;
-  while (blocks * share * 2 <= 2 * sms && share * 2 * groups <= rows + groups - 1) share *= 2;
+  while (tokens == 1 && blocks * share * 2 <= 2 * sms && share * groups < rows) share *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(blocks), unsigned(share)), cfg.blockDim = dim3(kThreads), cfg.stream = s;
-  cfg.dynamicSmemBytes = size_t(tokens) * (p.rot_dim / 2) * sizeof(float2);
+  cfg.dynamicSmemBytes = size_t(tokens) * (p.rot_dim / 2) * sizeof(float2) + (p.q_weight ? 2 * size_t(p.head_dim) * sizeof(float) : 0);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 1 : 0;
   uint32_t* status = device_status_ptr();
   Q27B_REQUIRE(status, "qk_rope: no device status word");
-  Q27B_CUDA(cudaLaunchKernelEx(&cfg, qk_rope_kernel<In, Out, kLanes>, p, tokens, status));
+  Q27B_CUDA(cudaLaunchKernelEx(&cfg, qk_rope_kernel<In, Out, kUnit, kLanes>, p, tokens, status));
   return 0;
 }
 
+// Whether a tensor can be loaded and stored `unit` channels at a time: base and strides in whole groups. Null passes.
+bool grouped(int unit, const void* base, int dtype, int64_t ld0, int64_t ld1, int64_t ld2 = 0) {
+  return reinterpret_cast<uintptr_t>(base) % std::min<size_t>(16, unit * type_size(dtype)) == 0 && ld0 % unit == 0 && ld1 % unit == 0 && ld2 % unit == 0;
+}
+bool all_grouped(int unit, const Args& p) {
+  return grouped(unit, p.q, p.in_dtype, p.q_ld_token, p.q_ld_head) && grouped(unit, p.k, p.in_dtype, p.k_ld_token, p.k_ld_head) &&
+         grouped(unit, p.v, p.in_dtype, p.v_ld_token, p.v_ld_head) && grouped(unit, p.q_out, p.out_dtype, p.q_out_ld_token, p.q_out_ld_head) &&
+         grouped(unit, p.k_out, p.out_dtype, p.k_out_ld_token, p.k_out_ld_head) &&
+         grouped(unit, p.k_cache, p.out_dtype, p.kc_ld_page, p.kc_ld_head, p.kc_ld_slot) &&
+         grouped(unit, p.v_cache, p.out_dtype, p.vc_ld_page, p.vc_ld_head, p.vc_ld_slot);
+}
+
+// Sixteen channels to a lane where sizes and strides allow (half the index arithmetic per byte, 16-byte accesses of 16-bit
+// types), else eight, with a whole warp to a row.
 template <typename In, typename Out>
 int launch_lanes(const Args& p, cudaStream_t s) {
-  if (p.head_dim <= 64) return launch<In, Out, 8>(p, s);
-  if (p.head_dim <= 128) return launch<In, Out, 16>(p, s);
-  return launch<In, Out, 32>(p, s);
+  if (p.head_dim % 16 || p.rot_dim % 16 || !all_grouped(8, p)) return launch<In, Out, 4, 32>(p, s);
+  if (p.head_dim <= 64) return launch<In, Out, 8, 4>(p, s);
+  if (p.head_dim <= 128) return launch<In, Out, 8, 8>(p, s);
+  return launch<In, Out, 8, 16>(p, s);
 }
 
 template <typename In>
@@ -216,11 +260,6 @@ int launch_out(const Args& p, cudaStream_t s) {
   if (p.out_dtype == Q27B_F32) return launch_lanes<In, float>(p, s);
   if (p.out_dtype == Q27B_BF16) return launch_lanes<In, __nv_bfloat16>(p, s);
   return launch_lanes<In, __half>(p, s);
-}
-
-// A tensor whose rows are loaded and stored four channels at a time: base and strides in whole groups of four.
-bool grouped(const void* base, int dtype, int64_t ld0, int64_t ld1, int64_t ld2 = 0) {
-  return base && (reinterpret_cast<uintptr_t>(base) % (4 * type_size(dtype))) == 0 && ld0 % 4 == 0 && ld1 % 4 == 0 && ld2 % 4 == 0;
 }
 
 }  // namespace
@@ -266,26 +305,26 @@ int q27b_qk_norm_rope(const q27b_qk_rope* a, void* stream) {
   Q27B_REQUIRE(p.in_dtype >= 0 && p.in_dtype <= 2 && p.out_dtype >= 0 && p.out_dtype <= 2, "qk_norm_rope: unknown type");
   if (p.T == 0) return 0;
   Q27B_REQUIRE(p.positions && p.turns, "qk_norm_rope: null positions or frequencies");
-  Q27B_REQUIRE(grouped(p.q, p.in_dtype, p.q_ld_token, p.q_ld_head) && grouped(p.q_out, p.out_dtype, p.q_out_ld_token, p.q_out_ld_head),
+  Q27B_REQUIRE(p.q && p.q_out && grouped(4, p.q, p.in_dtype, p.q_ld_token, p.q_ld_head) && grouped(4, p.q_out, p.out_dtype, p.q_out_ld_token, p.q_out_ld_head),
                "qk_norm_rope: q and q_out must not be null and must start and stride in whole groups of four channels");
   Q27B_REQUIRE(!p.q_weight == !p.k_weight || p.k_heads == 0, "qk_norm_rope: the norm needs both weights");
   if (p.q_weight) {
     const int wt = p.weight_f32 ? Q27B_F32 : Q27B_BF16;
-    Q27B_REQUIRE(grouped(p.q_weight, wt, 0, 0) && (p.k_heads == 0 || grouped(p.k_weight, wt, 0, 0)), "qk_norm_rope: the weights must be aligned to four values");
+    Q27B_REQUIRE(grouped(4, p.q_weight, wt, 0, 0) && (p.k_heads == 0 || grouped(4, p.k_weight, wt, 0, 0)), "qk_norm_rope: the weights must be aligned to four values");
     Q27B_REQUIRE(p.eps >= 0.f, "qk_norm_rope: eps must not be negative");
   }
   Q27B_REQUIRE(p.k_heads > 0 || (!p.k && !p.v && !p.slots), "qk_norm_rope: keys, values or slots without key heads");
   if (p.k_heads > 0) {
-    Q27B_REQUIRE(grouped(p.k, p.in_dtype, p.k_ld_token, p.k_ld_head), "qk_norm_rope: k must not be null and must start and stride in whole groups of four channels");
-    Q27B_REQUIRE(!p.v || (p.slots && grouped(p.v, p.in_dtype, p.v_ld_token, p.v_ld_head)),
+    Q27B_REQUIRE(p.k && grouped(4, p.k, p.in_dtype, p.k_ld_token, p.k_ld_head), "qk_norm_rope: k must not be null and must start and stride in whole groups of four channels");
+    Q27B_REQUIRE(!p.v || (p.slots && grouped(4, p.v, p.in_dtype, p.v_ld_token, p.v_ld_head)),
                  "qk_norm_rope: v goes into the cache only, and must start and stride in whole groups of four channels");
     if (p.slots) {
       Q27B_REQUIRE(!p.k_out, "qk_norm_rope: keys go either to k_out or into the cache");
-      Q27B_REQUIRE(p.page_size > 0 && p.pages > 0 && grouped(p.k_cache, p.out_dtype, p.kc_ld_page, p.kc_ld_head, p.kc_ld_slot) &&
-                       (!p.v || grouped(p.v_cache, p.out_dtype, p.vc_ld_page, p.vc_ld_head, p.vc_ld_slot)),
+      Q27B_REQUIRE(p.page_size > 0 && p.pages > 0 && p.k_cache && grouped(4, p.k_cache, p.out_dtype, p.kc_ld_page, p.kc_ld_head, p.kc_ld_slot) &&
+                       (!p.v || (p.v_cache && grouped(4, p.v_cache, p.out_dtype, p.vc_ld_page, p.vc_ld_head, p.vc_ld_slot))),
                    "qk_norm_rope: the cache must not be null or empty and must start and stride in whole groups of four channels");
     } else {
-      Q27B_REQUIRE(grouped(p.k_out, p.out_dtype, p.k_out_ld_token, p.k_out_ld_head),
+      Q27B_REQUIRE(p.k_out && grouped(4, p.k_out, p.out_dtype, p.k_out_ld_token, p.k_out_ld_head),
                    "qk_norm_rope: k_out must not be null and must start and stride in whole groups of four channels");
     }
   }

@@ -30,7 +30,7 @@ class KvCache:
             raise ValueError("KvCache: the channels of a head must be contiguous")
         if k.dtype not in (torch.bfloat16, torch.float16):
             raise ValueError(f"KvCache: the type must be bf16 or fp16, got {k.dtype}")
-        self.k, self.v = k, v
+        self.k, self.v, self.dtype = k, v, k.dtype
         self.pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.k_packed = (k.data_ptr(), *k.stride()[:3])
         self.v_packed = (v.data_ptr(), *v.stride()[:3])
@@ -70,36 +70,49 @@ class Attention:
         tokens in the cache, the new ones among them; q_begin int32 [B + 1]: rows of each sequence, None for one row each. max_new,
         max_kv: the longest sequence's rows and length as far as the host knows them; they only steer the split of the work.
         lse: an fp32 [T, heads] tensor that receives ln sum exp(scale q k). Rows in no sequence are not written."""
-        if q.dim() != 3 or q.shape[1] != self.heads or q.shape[2] != self.head_dim or q.stride(2) != 1:
-            raise ValueError(f"attention: q must be [T, {self.heads}, {self.head_dim}] with contiguous channels, got {list(q.shape)}")
+        if q.dim() != 3 or q.shape[1] != self.heads or q.shape[2] != self.head_dim:
+            raise ValueError(f"attention: q must be [T, {self.heads}, {self.head_dim}], got {list(q.shape)}")
         T, B = q.shape[0], kv_lens.shape[0]
         dev = device_of("attention", q, cache.k, table, kv_lens, q_begin, out, lse)
-        if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim or cache.k.dtype != q.dtype:
-            raise ValueError(f"attention: the cache holds {cache.kv_heads} heads of {cache.head_dim} channels in {cache.k.dtype}, the layer has {self.kv_heads} of {self.head_dim} and q is {q.dtype}")
-        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != B or (table.shape[1] > 1 and table.stride(1) != 1):
+        dtype = q.dtype
+        if cache.kv_heads != self.kv_heads or cache.head_dim != self.head_dim or cache.dtype is not dtype:
+            raise ValueError(f"attention: the cache holds {cache.kv_heads} heads of {cache.head_dim} channels in {cache.dtype}, the layer has {self.kv_heads} of {self.head_dim} and q is {dtype}")
+        if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != B or (table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError(f"attention: the table must be int32 [{B}, width] with contiguous rows")
-        if kv_lens.dtype != torch.int32 or kv_lens.dim() != 1 or not kv_lens.is_contiguous():
+        if kv_lens.dtype is not torch.int32 or kv_lens.dim() != 1 or not kv_lens.is_contiguous():
             raise ValueError("attention: kv_lens must be int32 [B], contiguous")
-        if q_begin is not None and (q_begin.dtype != torch.int32 or q_begin.shape != (B + 1,) or not q_begin.is_contiguous()):
+        if q_begin is not None and (q_begin.dtype is not torch.int32 or q_begin.shape != (B + 1,) or not q_begin.is_contiguous()):
             raise ValueError(f"attention: q_begin must be int32 [{B + 1}], contiguous")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
-            raise ValueError(f"attention: out must be {list(q.shape)} in {q.dtype} with contiguous channels")
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (T, self.heads) or not lse.is_contiguous()):
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape or out.dtype is not dtype:
+            raise ValueError(f"attention: out must be {list(q.shape)} in {dtype}")
+        if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (T, self.heads) or not lse.is_contiguous()):
             raise ValueError(f"attention: lse must be fp32 [{T}, {self.heads}], contiguous")
+        q0, q1, q2 = q.stride()
+        o0, o1, o2 = out.stride()
+        if q2 != 1 or o2 != 1:
+            raise ValueError("attention: the channels of q and out must be contiguous")
         width = table.shape[1]
         if max_new is None:
             max_new = 1 if q_begin is None else T
         if max_kv is None:
             max_kv = width * cache.page_size
-        head = (DTYPES[q.dtype], B, T, self.heads, self.kv_heads, self.head_dim, cache.page_size, cache.pages, width, self.window, self.sinks,
+        head = (DTYPES.get(dtype, -1), B, T, self.heads, self.kv_heads, self.head_dim, cache.page_size, cache.pages, width, self.window, self.sinks,
                 max(int(max_new), 1), max(int(max_kv), 1), self.scale, table.stride(0), table.data_ptr(), kv_lens.data_ptr(),
-                0 if q_begin is None else q_begin.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), *cache.k_packed, *cache.v_packed,
-                out.data_ptr(), out.stride(0), out.stride(1), 0 if lse is None else lse.data_ptr())
+                0 if q_begin is None else q_begin.data_ptr(), q.data_ptr(), q0, q1, *cache.k_packed, *cache.v_packed,
+                out.data_ptr(), o0, o1, 0 if lse is None else lse.data_ptr())
+        if dev.index != torch.cuda.current_device():
+            with torch.cuda.device(dev):
+                self._run(head, q, dev)
+        else:
+            self._run(head, q, dev)
+        return out
+
+    @staticmethod
+    def _run(head, q, dev):
         need = ctypes.c_size_t()
         call("q27b_attention_workspace", ATTENTION.pack(*head, 0, 0), ctypes.byref(need))
         # scratch of this call alone: torch's allocator keeps it apart from other streams' calls and other graphs' replays
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+        ws = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
         launch("q27b_paged_attention", ATTENTION.pack(*head, 0 if ws is None else ws.data_ptr(), need.value), dev)
-        return out

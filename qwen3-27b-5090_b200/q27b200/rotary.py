@@ -16,7 +16,7 @@ SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # Q27B_F32, Q27B_BF16, Q27B_F16
 # q27b_qk_rope (include/q27b200/capi.h), field by field
 QK_ROPE = struct.Struct("@11i2f" + "PPPP" + "Pqq" * 5 + "P2i" + "Pqqq" * 2)
-_NONE3 = (0, 0, 0)
+_NONE3, _NONE4 = (0, 0, 0), (0, 0, 0, 0)
 
 
 def device_of(what: str, *tensors: torch.Tensor) -> torch.device:
@@ -32,11 +32,13 @@ def device_of(what: str, *tensors: torch.Tensor) -> torch.device:
 
 def launch(name: str, packed: bytes, dev: torch.device):
     """The C entry on the device's current stream; the device is made current for the call where it is not."""
-    if dev.index == torch.cuda.current_device():
-        call(name, packed, torch.cuda.current_stream(dev).cuda_stream)
+    index = dev.index
+    if index == torch.cuda.current_device():
+        # (the raw handle: making a Stream object of it costs as much as the launch)
+        call(name, packed, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
-            call(name, packed, torch.cuda.current_stream(dev).cuda_stream)
+            call(name, packed, torch._C._cuda_getCurrentRawStream(index))
 
 
 class Rotary:
@@ -56,72 +58,72 @@ class Rotary:
         self.amplitude = float(a.value if amplitude is None else amplitude)
         signed = [t - (1 << 64) if t >> 63 else t for t in turns]
         self.turns = torch.tensor(signed, dtype=torch.int64, device=device)
+        self.turns_ptr = self.turns.data_ptr()
 
 
-def _heads(what: str, x: torch.Tensor, T: int, D: int, heads: int | None = None):
-    if x.dim() != 3 or x.shape[0] != T or x.shape[2] != D or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"{what}: expected [{T}, {'heads' if heads is None else heads}, {D}], got {list(x.shape)}")
-    if x.stride(2) != 1 and D > 1:
+def _heads(what: str, x: torch.Tensor, T: int, heads: int, D: int):
+    """Base and strides of [T, heads, D] with contiguous channels."""
+    if x.shape != (T, heads, D):
+        raise ValueError(f"{what}: expected [{T}, {heads}, {D}], got {list(x.shape)}")
+    a, b, c = x.stride()
+    if c != 1 and D > 1:
         raise ValueError(f"{what}: the channels of a head must be contiguous")
+    return x.data_ptr(), a, b
+
+
+def _new(like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def _launch(what, rotary, positions, q, k, v, q_out, k_out, q_weight, k_weight, eps, zero_centred, cache, slots):
-    if q.dim() != 3:
-        raise ValueError(f"{what}: q must be [tokens, heads, channels], got {list(q.shape)}")
+    if q.dim() != 3 or (k is not None and k.dim() != 3):
+        raise ValueError(f"{what}: q and k must be [tokens, heads, channels]")
     T, Hq, D = q.shape
     dev = device_of(what, q, positions, rotary.turns, k, v, q_out, k_out, q_weight, k_weight, slots, cache.k if cache else None)
-    _heads(what + ": q", q, T, D)
-    if q.dtype not in DTYPES:
-        raise ValueError(f"{what}: q must be fp32, bf16 or fp16, got {q.dtype}")
-    if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (T,) or not positions.is_contiguous():
+    dtype, out_dtype, pos_dtype = q.dtype, q_out.dtype, positions.dtype
+    if dtype not in DTYPES or out_dtype not in DTYPES:
+        raise ValueError(f"{what}: inputs and outputs must be fp32, bf16 or fp16, got {dtype} and {out_dtype}")
+    if (pos_dtype is not torch.int64 and pos_dtype is not torch.int32) or positions.shape != (T,) or not positions.is_contiguous():
         raise ValueError(f"{what}: positions must be int64 or int32 [{T}], contiguous")
-    Hk = 0
+    qp, qo = _heads(what + ": q", q, T, Hq, D), _heads(what + ": q_out", q_out, T, Hq, D)
+    Hk, kp, vp, ko = 0, _NONE3, _NONE3, _NONE3
     if k is not None:
-        Hk = k.shape[1] if k.dim() == 3 else 0
-        _heads(what + ": k", k, T, D)
+        Hk = k.shape[1]
+        kp = _heads(what + ": k", k, T, Hk, D)
         if v is not None:
-            _heads(what + ": v", v, T, D, Hk)
-        if any(x is not None and x.dtype != q.dtype for x in (k, v)):
+            vp = _heads(what + ": v", v, T, Hk, D)
+        if k.dtype is not dtype or (v is not None and v.dtype is not dtype):
             raise ValueError(f"{what}: q, k and v must have one type")
-    _heads(what + ": q_out", q_out, T, D, Hq)
+    qw = kw = 0
+    weight_f32 = False
     if q_weight is not None:
-        if q_weight.dtype not in (torch.float32, torch.bfloat16) or any(w is not None and (w.dtype != q_weight.dtype or w.shape != (D,) or not w.is_contiguous()) for w in (q_weight, k_weight)):
+        weight_f32 = q_weight.dtype is torch.float32
+        if not (weight_f32 or q_weight.dtype is torch.bfloat16) or any(w.dtype is not q_weight.dtype or w.shape != (D,) or not w.is_contiguous() for w in (q_weight, k_weight)):
             raise ValueError(f"{what}: the norm weights must be fp32 or bf16 [{D}], contiguous, of one type")
-    ko = kc = vc = None
-    page_size = pages = 0
+        qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
+    slot_ptr, page_size, pages, kc, vc = 0, 0, 0, _NONE4, _NONE4
     if cache is not None:
-        if slots is None or slots.dtype != torch.int64 or slots.shape != (T,) or not slots.is_contiguous():
+        if slots is None or slots.dtype is not torch.int64 or slots.shape != (T,) or not slots.is_contiguous():
             raise ValueError(f"{what}: slots must be int64 [{T}], contiguous")
-        if cache.kv_heads != Hk or cache.head_dim != D or cache.k.dtype != q_out.dtype:
-            raise ValueError(f"{what}: the cache holds {cache.kv_heads} heads of {cache.head_dim} channels in {cache.k.dtype}, got {Hk} of {D} for {q_out.dtype}")
-        kc, vc = cache.k_packed, cache.v_packed
-        page_size, pages = cache.page_size, cache.pages
+        if cache.kv_heads != Hk or cache.head_dim != D or cache.dtype is not out_dtype:
+            raise ValueError(f"{what}: the cache holds {cache.kv_heads} heads of {cache.head_dim} channels in {cache.dtype}, got {Hk} of {D} for {out_dtype}")
+        slot_ptr, page_size, pages, kc, vc = slots.data_ptr(), cache.page_size, cache.pages, cache.k_packed, cache.v_packed
     elif k is not None:
-        _heads(what + ": k_out", k_out, T, D, Hk)
-        if k_out.dtype != q_out.dtype:
+        ko = _heads(what + ": k_out", k_out, T, Hk, D)
+        if k_out.dtype is not out_dtype:
             raise ValueError(f"{what}: q_out and k_out must have one type")
-        ko = (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
-    if q_out.dtype not in DTYPES:
-        raise ValueError(f"{what}: outputs must be fp32, bf16 or fp16, got {q_out.dtype}")
-    packed = QK_ROPE.pack(
-        T, Hq, Hk, D, rotary.rot_dim, rotary.interleaved, DTYPES[q.dtype], DTYPES[q_out.dtype], positions.dtype == torch.int64,
-        q_weight is not None and q_weight.dtype == torch.float32, zero_centred, eps, rotary.amplitude,
-        positions.data_ptr(), rotary.turns.data_ptr(), 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
-        q.data_ptr(), q.stride(0), q.stride(1),
-        *(_NONE3 if k is None else (k.data_ptr(), k.stride(0), k.stride(1))),
-        *(_NONE3 if v is None else (v.data_ptr(), v.stride(0), v.stride(1))),
-        q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *(ko or _NONE3),
-        0 if cache is None else slots.data_ptr(), page_size, pages, *(kc or (0, 0, 0, 0)), *(vc or (0, 0, 0, 0)))
-    launch("q27b_qk_norm_rope", packed, dev)
+    launch("q27b_qk_norm_rope", QK_ROPE.pack(
+        T, Hq, Hk, D, rotary.rot_dim, rotary.interleaved, DTYPES[dtype], DTYPES[out_dtype], pos_dtype is torch.int64, weight_f32, zero_centred, eps,
+        rotary.amplitude, positions.data_ptr(), rotary.turns_ptr, qw, kw, *qp, *kp, *vp, *qo, *ko, slot_ptr, page_size, pages, *kc, *vc), dev)
 
 
 def rope(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
          k_out: torch.Tensor | None = None):
     """Rotates q [T, heads, D] (and k [T, kv_heads, D]) by positions [T]; returns (q_out, k_out). The outputs may be the inputs
     themselves; without them new tensors of the inputs' type are made."""
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    q_out = _new(q, q.dtype) if q_out is None else q_out
     if k is not None and k_out is None:
-        k_out = torch.empty(k.shape, dtype=q_out.dtype, device=k.device)
+        k_out = _new(k, q_out.dtype)
     _launch("rope", rotary, positions, q, k, None, q_out, k_out, None, None, 0.0, False, None, None)
     return q_out, k_out
 
@@ -140,8 +142,8 @@ def qk_norm_rope(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: to
     if q_weight is None or k_weight is None or k is None:
         raise ValueError("qk_norm_rope: k and both weights are needed (rope rotates without the norm)")
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=cache.k.dtype if cache is not None else dtype or q.dtype, device=q.device)
+        q_out = _new(q, cache.dtype if cache is not None else dtype or q.dtype)
     if cache is None and k_out is None:
-        k_out = torch.empty(k.shape, dtype=q_out.dtype, device=k.device)
+        k_out = _new(k, q_out.dtype)
     _launch("qk_norm_rope", rotary, positions, q, k, v, q_out, k_out, q_weight, k_weight, float(eps), zero_centred, cache, slots)
     return q_out if cache is not None else (q_out, k_out)

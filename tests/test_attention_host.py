@@ -167,7 +167,7 @@ def test_python_refusals():
         rope(r, pos, q)
     with pytest.raises(ValueError, match="CUDA device"):
         Attention(4, 2, 64)(q, cache, table, torch.zeros(1, dtype=torch.int32))
-    with pytest.raises(ValueError, match="contiguous channels"):
+    with pytest.raises(ValueError, match="must be .T, 4, 32"):
         Attention(4, 2, 32)(q, cache, table, torch.zeros(1, dtype=torch.int32))
     w = torch.zeros(64)
     for kw in (dict(v=q[:, :2]), dict(slots=pos), dict(cache=cache, k_out=q[:, :2])):
