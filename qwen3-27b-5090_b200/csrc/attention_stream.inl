@@ -177,67 +177,57 @@ __global__ void __launch_bounds__(kStreamThreads, StreamCfg<D>::kCtasPerSm)
 
   if (warp == 4) {
     // ---- producer ----------------------------------------------------------------------------------------------------
-    const int box = min(p.page_size, kStreamKeys);           // keys of one copy
-    const uint32_t box_bytes = uint32_t(box) * 128u;         // per 64 channels
+    // Lane x looks after box x of a tile: it looks its page up (a tile ahead: the table's latency would add to the copy's) and
+    // issues its copies.
+    const int box = min(p.page_size, kStreamKeys), boxes = kStreamKeys / box;
+    const uint32_t box_bytes = uint32_t(box) * 128u;  // per 64 channels
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool stop = false;  // a wait ran out (the same in all lanes)
-    int held_b = -1, held_from = 0, held = 0, ahead = 0;  // page-table entries, one per lane: 32 from held_from, and the next 32
-    for (int64_t t = t0; t < t1 && cur.b < p.B; cur.next(p, max_rows)) {
-      const StreamSeq& q = cur.q;
-      const int end = int(min(int64_t(q.tiles), cur.i + (t1 - t)));
-      const int reach = min(q.s.len, q.s.reach);
-      for (; cur.i < end; cur.i++, t++) {
-        const int key0 = q.tile(cur.i) * kStreamKeys;
+    struct Box {
+      int k0, page;
+      bool need;
+    };
+    auto look_up = [&](const StreamCursor& at, int i) {
+      const int reach = min(at.q.s.len, at.q.s.reach);
+      Box x;
+      x.k0 = at.q.tile(i) * kStreamKeys + lane * box, x.page = 0;
+      x.need = lane < boxes && x.k0 < reach && (x.k0 < p.sinks || min(x.k0 + box, reach) > at.q.low);  // pages that no row sees are not read
+      if (x.need) x.page = p.table[at.b * p.table_ld + x.k0 / p.page_size];
+      return x;
+    };
+    Box next = look_up(cur, cur.i);
+    for (int64_t t = t0; t < t1 && cur.b < p.B && !stop;) {
+      const int end = int(min(int64_t(cur.q.tiles), cur.i + (t1 - t))), hk = cur.hk;
+      if (cur.q.s.len > cur.q.s.reach && lane == 0) atomicCAS(status, 0u, uint32_t(kStatusBadPage));
+      for (int i = cur.i; i < end; i++, t++) {
+        const Box x = next;
+        if (i + 1 < end) {
+          next = look_up(cur, i + 1);
+        } else {
+          cur.next(p, max_rows);
+          if (t + 1 < t1 && cur.b < p.B) next = look_up(cur, 0);
+        }
+        int page = x.page;
+        if (x.need && (page < 0 || page >= p.pages)) page = p.pages, atomicCAS(status, 0u, uint32_t(kStatusBadPage));  // (reads zeros)
+        const uint32_t bytes = uint32_t(__popc(__ballot_sync(0xffffffffu, x.need))) * 2 * (D / 64) * box_bytes;
         if (issued >= C::kStages && !warp_wait(empty(stage), phase ^ 1u, &abort_flag, status, kStatusEmptyWaitTimeout, 0)) {
           stop = true;
           break;
         }
-        uint32_t bytes = 0;
-        int page_at[4] = {};
-        bool need[4];
+        if (lane == 0) mbar_arrive_expect_tx(full(stage), bytes);
+        __syncwarp();
+        if (x.need) {
+          const uint32_t kdst = base + stage * 2 * C::kTileBytes + lane * box_bytes, vdst = kdst + C::kTileBytes;
+          const int slot = x.k0 % p.page_size;
 #pragma unroll
-        for (int x = 0; x < 4; x++) {  // copies of this tile: at most 64 / 16
-          const int k0 = key0 + x * box, k1 = min(k0 + box, reach);
-          // a page that no row of the sequence sees is not read
-          need[x] = x * box < kStreamKeys && k0 < reach && (k0 < p.sinks || k1 > q.low);
-          if (!need[x]) continue;
-          const int at = k0 / p.page_size;
-          if (held_b != cur.b || at < held_from || at >= held_from + 64) {
-            held_b = cur.b, held_from = at;
-            const int32_t* row = p.table + cur.b * p.table_ld;
-            held = at + lane < p.table_width ? row[at + lane] : -1;
-            ahead = at + 32 + lane < p.table_width ? row[at + 32 + lane] : -1;
-          } else if (at >= held_from + 32) {
-            held_from += 32, held = ahead;
-            ahead = held_from + 32 + lane < p.table_width ? p.table[cur.b * p.table_ld + held_from + 32 + lane] : -1;
-          }
-          int page = __shfl_sync(0xffffffffu, held, at - held_from);
-          if (page < 0 || page >= p.pages) {  // no such page: the copy reads zeros from behind the cache's end
-            page = p.pages;
-            if (lane == 0) atomicCAS(status, 0u, uint32_t(kStatusBadPage));
-          }
-          page_at[x] = page;
-          bytes += 2 * (D / 64) * box_bytes;
-        }
-        if (lane == 0) {
-          mbar_arrive_expect_tx(full(stage), bytes);
-          const uint32_t kdst = base + stage * 2 * C::kTileBytes, vdst = kdst + C::kTileBytes;
+          for (int d = 0; d < D / 64; d++) tma_load_4d(kdst + d * kStreamKeys * 128, &kmap, d * 64, slot, hk, page, full(stage));
 #pragma unroll
-          for (int x = 0; x < 4; x++) {
-            if (!need[x]) continue;
-            const int slot = (key0 + x * box) % p.page_size;
-#pragma unroll
-            for (int d = 0; d < D / 64; d++) tma_load_4d(kdst + d * kStreamKeys * 128 + x * box_bytes, &kmap, d * 64, slot, cur.hk, page_at[x], full(stage));
-#pragma unroll
-            for (int d = 0; d < D / 64; d++) tma_load_4d(vdst + d * kStreamKeys * 128 + x * box_bytes, &vmap, d * 64, slot, cur.hk, page_at[x], full(stage));
-          }
+          for (int d = 0; d < D / 64; d++) tma_load_4d(vdst + d * kStreamKeys * 128, &vmap, d * 64, slot, hk, page, full(stage));
         }
         issued++;
         if (++stage == C::kStages) stage = 0, phase ^= 1u;
       }
-      if (cur.b < p.B && q.s.len > q.s.reach && lane == 0) atomicCAS(status, 0u, uint32_t(kStatusBadPage));
-      if (stop) break;
     }
     if (stop) {  // unwinding: no copy may still be in flight when the CTA ends
       for (int s = 0; s < C::kStages && s < issued; s++) {

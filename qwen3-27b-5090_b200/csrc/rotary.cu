@@ -105,7 +105,7 @@ __device__ __forceinline__ void turn_pair(float& a, float& b, float2 cs) {
 
 // kLanes lanes to a row, kUnit * 2 channels (kUnit pairs, or two runs that do not turn) to a lane; `tokens` tokens to a CTA.
 template <typename In, typename Out, int kUnit, int kLanes>
-__global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant__ Args p, int tokens, uint32_t* status) {
+__global__ void __launch_bounds__(kThreads, 4) qk_rope_kernel(const __grid_constant__ Args p, int tokens, uint32_t* status) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int D = p.head_dim, pairs = p.rot_dim / 2, t0 = blockIdx.x * tokens, nt = min(tokens, p.T - t0);
   float2* table = reinterpret_cast<float2*>(smem);                   // [tokens][pairs] (cos, sin)
@@ -114,6 +114,24 @@ __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant
   const bool norm = p.q_weight != nullptr;
   pdl_wait();
   pdl_trigger();
+  // The CTA's row groups are dealt out to its tokens; a group walks the heads of its token (q, then k, then v).
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, per_token = kThreads / kLanes / tokens;
+  const int tl = group / per_token, t = t0 + tl, step = per_token * gridDim.y;
+  const int qk_heads = p.q_heads + p.k_heads, rows = qk_heads + (p.v ? p.k_heads : 0);
+  const bool active = lane * 2 * kUnit < D && tl < nt, turns = lane * 2 * kUnit < p.rot_dim;
+  int a, b;  // the two runs of kUnit channels of this lane
+  if (p.interleaved || !turns)
+    a = lane * 2 * kUnit, b = a + kUnit;
+  else
+    a = lane * kUnit, b = pairs + lane * kUnit;
+  auto source = [&](int head) {
+    return head < p.q_heads ? static_cast<const In*>(p.q) + t * p.q_ld_token + head * p.q_ld_head
+           : head < qk_heads ? static_cast<const In*>(p.k) + t * p.k_ld_token + (head - p.q_heads) * p.k_ld_head
+                             : static_cast<const In*>(p.v) + t * p.v_ld_token + (head - qk_heads) * p.v_ld_head;
+  };
+  Raw<In, kUnit> next[2];
+  int head = blockIdx.y * per_token + group % per_token;  // (the first row is on its way while the tables are made)
+  if (active && head < rows) next[0].load(source(head) + a), next[1].load(source(head) + b);
   for (int i = threadIdx.x; i < nt * pairs; i += kThreads) {
     const int t = t0 + i / pairs;
     const int64_t pos = p.pos64 ? static_cast<const int64_t*>(p.positions)[t] : int64_t(static_cast<const int32_t*>(p.positions)[t]);
@@ -133,29 +151,11 @@ __global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant
   }
   __syncthreads();
 
-  // The CTA's row groups are dealt out to its tokens; a group walks the heads of its token (q, then k, then v).
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, per_token = kThreads / kLanes / tokens;
-  const int tl = group / per_token, t = t0 + tl, step = per_token * gridDim.y;
-  const int qk_heads = p.q_heads + p.k_heads, rows = qk_heads + (p.v ? p.k_heads : 0);
-  const bool active = lane * 2 * kUnit < D && tl < nt, turns = lane * 2 * kUnit < p.rot_dim;
-  int a, b;  // the two runs of kUnit channels of this lane
-  if (p.interleaved || !turns)
-    a = lane * 2 * kUnit, b = a + kUnit;
-  else
-    a = lane * kUnit, b = pairs + lane * kUnit;
   float2 cs[kUnit];
   if (active && turns) {
 #pragma unroll
     for (int i = 0; i < kUnit; i++) cs[i] = table[tl * pairs + lane * kUnit + i];
   }
-  auto source = [&](int head) {
-    return head < p.q_heads ? static_cast<const In*>(p.q) + t * p.q_ld_token + head * p.q_ld_head
-           : head < qk_heads ? static_cast<const In*>(p.k) + t * p.k_ld_token + (head - p.q_heads) * p.k_ld_head
-                             : static_cast<const In*>(p.v) + t * p.v_ld_token + (head - qk_heads) * p.v_ld_head;
-  };
-  Raw<In, kUnit> next[2];
-  int head = blockIdx.y * per_token + group % per_token;
-  if (active && head < rows) next[0].load(source(head) + a), next[1].load(source(head) + b);
   const float inv_dim = 1.f / float(D);
   // (the loop runs equally often in all lanes of a warp: its shuffles are whole-warp)
   for (int h0 = blockIdx.y * per_token; h0 < rows; h0 += step, head += step) {
