@@ -378,7 +378,7 @@ typedef struct q27b_attention {
   int window, sinks;           /* window 0: none */
   int max_new, max_kv;         /* hints for the split of the work, at least 1: rows and length of the longest sequence. The
                                   results hold whatever they say. */
-  float scale;                 /* on q . k */
+  float scale;                 /* on q . k: finite, not negative */
   int64_t table_ld;
   const int32_t* table;        /* [B][table_width] */
   const int32_t* kv_lens;      /* [B] */

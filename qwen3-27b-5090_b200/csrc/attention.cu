@@ -5,6 +5,7 @@
 // j <= p with j > p - window or j < sinks. With s_j = scale q . k_j:  o = sum_j exp(s_j - m) v_j / l,  l = sum_j exp(s_j - m),
 // m the running maximum: one pass over the keys, in fp32.
 #include <algorithm>
+#include <cmath>
 
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -155,6 +156,7 @@ int check_sizes(const Args& p) {
                "attention: the cache and the table must not be empty, nor the table name 2^30 tokens or more (pages = %d, width = %d)", p.pages, p.table_width);
   Q27B_REQUIRE(int64_t(p.T) * p.heads < (int64_t(1) << 30), "attention: T x heads must stay below 2^30 (%d, %d)", p.T, p.heads);
   Q27B_REQUIRE(p.window >= 0 && p.sinks >= 0, "attention: window and sinks must not be negative");
+  Q27B_REQUIRE(p.scale >= 0.f && p.scale < INFINITY, "attention: the scale must be finite and not negative (%g)", double(p.scale));
   Q27B_REQUIRE(p.max_new >= 1 && p.max_kv >= 1, "attention: max_new and max_kv must be at least 1");
   return 0;
 }

@@ -177,8 +177,7 @@ __global__ void __launch_bounds__(kStreamThreads, StreamCfg<D>::kCtasPerSm)
 
   if (warp == 4) {
     // ---- producer ----------------------------------------------------------------------------------------------------
-    // Lane x looks after box x of a tile: it looks its page up (a tile ahead: the table's latency would add to the copy's) and
-    // issues its copies.
+    // Lane x looks up the page of box x of a tile, a tile ahead: the table's latency would add to the copy's.
     const int box = min(p.page_size, kStreamKeys), boxes = kStreamKeys / box;
     const uint32_t box_bytes = uint32_t(box) * 128u;  // per 64 channels
     int stage = 0, issued = 0;
@@ -210,20 +209,25 @@ __global__ void __launch_bounds__(kStreamThreads, StreamCfg<D>::kCtasPerSm)
         }
         int page = x.page;
         if (x.need && (page < 0 || page >= p.pages)) page = p.pages, atomicCAS(status, 0u, uint32_t(kStatusBadPage));  // (reads zeros)
-        const uint32_t bytes = uint32_t(__popc(__ballot_sync(0xffffffffu, x.need))) * 2 * (D / 64) * box_bytes;
+        const uint32_t needs = __ballot_sync(0xffffffffu, x.need);
         if (issued >= C::kStages && !warp_wait(empty(stage), phase ^ 1u, &abort_flag, status, kStatusEmptyWaitTimeout, 0)) {
           stop = true;
           break;
         }
-        if (lane == 0) mbar_arrive_expect_tx(full(stage), bytes);
-        __syncwarp();
-        if (x.need) {
-          const uint32_t kdst = base + stage * 2 * C::kTileBytes + lane * box_bytes, vdst = kdst + C::kTileBytes;
-          const int slot = x.k0 % p.page_size;
+        // one elected lane issues: copies issued by several lanes of a warp go out one lane at a time
+        const uint32_t bar = full(stage), dst = base + stage * 2 * C::kTileBytes;
+        const int key0 = __shfl_sync(0xffffffffu, x.k0, 0);
+        if (elect_one()) mbar_arrive_expect_tx(bar, uint32_t(__popc(needs)) * 2 * (D / 64) * box_bytes);
+        for (uint32_t left = needs; left; left &= left - 1) {
+          const int lane_of = __ffs(left) - 1, page_of = __shfl_sync(0xffffffffu, page, lane_of), slot = (key0 + lane_of * box) & (p.page_size - 1);
+          if (elect_one()) {
+            const uint32_t kdst = dst + lane_of * box_bytes, vdst = kdst + C::kTileBytes;
 #pragma unroll
-          for (int d = 0; d < D / 64; d++) tma_load_4d(kdst + d * kStreamKeys * 128, &kmap, d * 64, slot, hk, page, full(stage));
+            for (int d = 0; d < D / 64; d++) tma_load_4d(kdst + d * kStreamKeys * 128, &kmap, d * 64, slot, hk, page_of, bar);
 #pragma unroll
-          for (int d = 0; d < D / 64; d++) tma_load_4d(vdst + d * kStreamKeys * 128, &vmap, d * 64, slot, hk, page, full(stage));
+            for (int d = 0; d < D / 64; d++) tma_load_4d(vdst + d * kStreamKeys * 128, &vmap, d * 64, slot, hk, page_of, bar);
+          }
+          __syncwarp();
         }
         issued++;
         if (++stage == C::kStages) stage = 0, phase ^= 1u;

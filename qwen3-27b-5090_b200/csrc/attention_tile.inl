@@ -93,6 +93,9 @@ struct TileCursor {
   }
 };
 
+// Bits 0 .. n - 1.
+__device__ __forceinline__ uint64_t below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
+
 // The code of what seldom happens is laid out away from the loop, which is long enough to feel its instruction fetches.
 __device__ __forceinline__ bool rarely(bool x) { return __builtin_expect(x, 0); }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   // (the other warps are idle: they complete the warpgroup)
   if (warp == C::kSoftmaxWarps + NT) {
     // ---- copies -----------------------------------------------------------------------------------------------------------
-    const int boxes = C::kKeys / box;  // per tile: at most eight, one per lane
+    const int boxes = C::kKeys / box, page_bits = __ffs(p.page_size) - 1;  // boxes per tile: at most eight, one per lane
     int slot = 0, issued = 0;
     uint32_t phase = 0;
     bool stop = false;  // a wait ran out (the same in all lanes)
@@ -337,12 +340,12 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       x.k0 = x.tile0 + lane * box, x.page = 0;
       const int k1 = min(x.k0 + box, cur.r.reach);
       x.need = lane < boxes && x.k0 < cur.r.reach && (x.k0 < p.sinks || k1 > cur.r.low);
-      if (x.need) x.page = p.table[cur.b * p.table_ld + x.k0 / p.page_size];
+      if (x.need) x.page = p.table[cur.b * p.table_ld + (x.k0 >> page_bits)];
       return x;
     };
     auto load = [&](const CUtensorMap* map, bool values, const Box& x) {  // all lanes
       if (stop) return;
-      const int tile0 = x.tile0, k0 = x.k0;
+      const int tile0 = x.tile0;
       int page = x.page;
       if (x.need && (page < 0 || page >= p.pages)) page = p.pages, atomicCAS(status, 0u, uint32_t(kStatusBadPage));  // (reads zeros)
       const uint32_t needs = __ballot_sync(0xffffffffu, x.need);
@@ -357,11 +360,19 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
           stop = true;
           return;
         }
-        if (lane == 0) mbar_arrive_expect_tx(full(slot), uint32_t(__popc(in_part) * dn * box) * 128u);
-        __syncwarp();
-        if ((in_part >> lane) & 1u) {
-          const uint32_t dst = ring + slot * C::kSlotBytes + uint32_t((k0 - tile0) - (rows < C::kKeys ? part * rows : 0)) * 128u;
-          for (int d = 0; d < dn; d++) tma_load_4d(dst + d * rows * 128, map, (d0 + d) * 64, k0 % p.page_size, cur.hk, page, full(slot));
+        // One elected lane issues, with the boxes' pages from the lanes that looked them up: copies issued by several lanes of a
+        // warp go out one lane at a time, at 190 cycles each.
+        const uint32_t dst = ring + slot * C::kSlotBytes, bar = full(slot);
+        if (elect_one()) mbar_arrive_expect_tx(bar, uint32_t(__popc(in_part) * dn * box) * 128u);
+        for (uint32_t left = in_part; left; left &= left - 1) {
+          const int lane_of = __ffs(left) - 1, page_of = __shfl_sync(0xffffffffu, page, lane_of);
+          const int at = tile0 + lane_of * box, in_tile = lane_of * box - (rows < C::kKeys ? part * rows : 0);
+          if (elect_one()) {
+#pragma unroll
+            for (int d = 0; d < kBlocks; d++)
+              if (d < dn) tma_load_4d(dst + (d * rows + in_tile) * 128, map, (d0 + d) * 64, at & (p.page_size - 1), cur.hk, page_of, bar);
+          }
+          __syncwarp();
         }
         issued++;
         if (++slot == C::kSlots) slot = 0, phase ^= 1u;
@@ -513,36 +524,40 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
     // ---- softmax, scaling, epilogue: two threads per row, each with half the keys of S and half the channels of O ------------------
     const int tile = warp / 8, half = (warp / 4) % 2, row_in_tile = (warp % 4) * 32 + lane;
     const uint32_t lanes = uint32_t(32 * (warp % 4)) << 16, o_at = tmem + lanes + C::kO + tile * D + half * (D / 2);
-    const float c2 = fabsf(p.scale) * 1.4426950408889634f, scale_log2 = c2 > 0.f ? c2 : 1e-30f;  // (0 would turn a masked -infinity into NaN)
-    const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;  // a negative scale goes into the queries' signs
+    const float c2 = p.scale * 1.4426950408889634f, scale_log2 = c2 > 0.f ? c2 : 1e-30f;  // (0 would turn a masked -infinity into NaN)
     auto pair_bar = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + tile * 4 + warp % 4) : "memory"); };  // the two warps of 32 rows
     uint32_t s_phase = 0, pv_phase = 0;  // (bit b: of S buffer b)
     int chunk = 0;  // ring places used before this segment
-    // this thread's half of its row of the segment at `at` into shared memory, in the layout of the products' operands
+    // This thread's half of its row of the segment at `at` starts on its way into shared memory, in the layout of the products'
+    // operands (zeros for a row that is not there); q_here hands it over.
     auto load_q = [&](const TileCursor& at) {
       const int row = at.rt * C::kRows + tile * 128 + row_in_tile;
-      const uint16_t* src = static_cast<const uint16_t*>(p.q) + (at.s.row0 + row / G) * p.q_ld_token + (at.hk * G + row % G) * p.q_ld_head;
-      const uint32_t dst = base + tile * C::kQBytes + row_in_tile * 128;
       const bool live = row < at.rows;
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + (live ? (at.s.row0 + row / G) * p.q_ld_token + (at.hk * G + row % G) * p.q_ld_head : 0);
+      const uint32_t dst = base + tile * C::kQBytes + row_in_tile * 128;
 #pragma unroll
       for (int x = 0; x < D / 16; x++) {
         const int d = half * (D / 16) + x;
-        uint4 v = live ? reinterpret_cast<const uint4*>(src)[d] : make_uint4(0, 0, 0, 0);
-        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (d / 8) * 128 * 128 + (((d % 8) ^ (row_in_tile & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (d / 8) * 128 * 128 + (((d % 8) ^ (row_in_tile & 7)) << 4)), "l"(src + d * 8), "r"(live ? 16 : 0) : "memory");
       }
+    };
+    auto q_here = [&] {
+      asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready(tile));
     };
     auto in_use = [&](const TileCursor& at) { return at.rows - at.rt * C::kRows > tile * 128; };
-    if (work && cur.any(p, t1) && in_use(cur)) load_q(cur);
+    if (work && cur.any(p, t1) && in_use(cur)) load_q(cur), q_here();
     while (work && cur.any(p, t1)) {
       const int from = cur.from, end = cur.end(t1);
       auto load_next_q = [&](TileCursor nxt) {
         nxt.template next<C::kRows, C::kSegmentCost>(p, min_rows);
-        if (nxt.any(p, t1) && in_use(nxt)) load_q(nxt);
+        const bool any = nxt.any(p, t1) && in_use(nxt);
+        if (any) load_q(nxt);
+        return any;
       };
+      bool next_q = false;  // the next segment's Q is on its way
       if (in_use(cur)) {
         const int row = cur.rt * C::kRows + tile * 128 + row_in_tile, row_end = min(cur.rows, cur.rt * C::kRows + tile * 128 + 128);
         const int first = cur.s.len - cur.s.rows, pos = first + row / G;
@@ -561,6 +576,8 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
           const bool here = mbar_wait_bounded(s_full(buf), (s_phase >> buf) & 1u, &abort_flag, status, kStatusAccumWaitTimeout);
           s_phase ^= 1u << buf;
           tc_fence_after_sync();
+          // every product with this segment's Q has ended: the next segment's takes its place while the last softmax runs
+          if (rarely(i == end - 1)) next_q = load_next_q(cur);
           auto wait_pv = [&] {  // of the tile before (kTiles == 1): it may still be adding to O
             mbar_wait_bounded(pv_done(0), pv_phase ^ 1u, &abort_flag, status, kStatusAccumWaitTimeout);
             tc_fence_after_sync();
@@ -573,9 +590,12 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
               tmem_ld32(s_at, s), tmem_ld32(s_at + 32, s + 32);
               tmem_ld_wait();
               if (rarely(edge)) {
-                const int at = k0 + half * 64, hi = min(pos, cur.r.reach - 1) - at, lo = p.window > 0 ? pos - p.window + 1 - at : -1, si = p.sinks - at;
+                // bit x: this row sees key at + x
+                const int at = k0 + half * 64, hi = min(pos, cur.r.reach - 1) - at, lo = p.window > 0 ? pos - p.window + 1 - at : 0, si = p.sinks - at;
+                const uint64_t seen = below(hi + 1) & (~below(lo) | below(si));
+                const uint32_t seen0 = uint32_t(seen), seen1 = uint32_t(seen >> 32);
 #pragma unroll
-                for (int x = 0; x < 64; x++) s[x] = x <= hi && (x >= lo || x < si) ? s[x] : -INFINITY;
+                for (int x = 0; x < 32; x++) s[x] = (seen0 >> x) & 1u ? s[x] : -INFINITY, s[x + 32] = (seen1 >> x) & 1u ? s[x + 32] : -INFINITY;
                 tmem_st32(s_at, reinterpret_cast<uint32_t*>(s)), tmem_st32(s_at + 32, reinterpret_cast<uint32_t*>(s + 32));
                 tmem_st_wait();
               }
@@ -660,8 +680,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(p_ready(buf));
         }
-        // every product with this segment's Q has ended (its S was read): the next segment's may take its place
-        load_next_q(cur);
+        if (next_q) q_here();
         // the last product of the segment, then its result
         const bool done = mbar_wait_bounded(pv_done(tile), NT == 2 ? pv_phase : pv_phase ^ 1u, &abort_flag, status, kStatusAccumWaitTimeout);
         if (NT == 2) pv_phase ^= 1u;
@@ -702,8 +721,8 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
           }
           tc_fence_before_sync();
         }
-      } else {
-        load_next_q(cur);
+      } else if (load_next_q(cur)) {
+        q_here();
       }
       chunk += 2 * (end - from) * C::kParts;
       cur.template next<C::kRows, C::kSegmentCost>(p, min_rows);

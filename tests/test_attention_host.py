@@ -125,7 +125,7 @@ def attention_record(**change):
     ({"dtype": 0}, "bf16 or fp16"), ({"dtype": 7}, "bf16 or fp16"), ({"B": -1}, "bad counts"), ({"T": -2}, "bad counts"), ({"heads": 5}, "multiple of kv_heads"),
     ({"kv_heads": 0}, "multiple of kv_heads"), ({"heads": 0}, "multiple of kv_heads"), ({"head_dim": 96}, "head_dim"), ({"page_size": 48}, "page_size"), ({"page_size": 8}, "page_size"),
     ({"pages": 0}, "must not be empty"), ({"table_width": 0}, "must not be empty"), ({"table_width": 1 << 27}, "2\\^30"), ({"window": -1}, "negative"), ({"sinks": -1}, "negative"),
-    ({"max_new": 0}, "at least 1"), ({"max_kv": 0}, "at least 1"), ({"T": 3}, "one row per sequence"), ({"table": 0}, "null table"), ({"kv_lens": 0}, "null table"),
+    ({"scale": -0.1}, "scale"), ({"scale": float("nan")}, "scale"), ({"scale": float("inf")}, "scale"), ({"max_new": 0}, "at least 1"), ({"max_kv": 0}, "at least 1"), ({"T": 3}, "one row per sequence"), ({"table": 0}, "null table"), ({"kv_lens": 0}, "null table"),
     ({"q": 0}, "q and out"), ({"q": (1 << 20) + 8}, "q and out"), ({"out": 0}, "q and out"), ({"out_ld_head": 68}, "q and out"),
     ({"k_cache": 0}, "cache must not be null"), ({"v_cache": (1 << 20) + 2}, "cache must not be null"), ({"kc_ld_slot": 60}, "cache must not be null"), ({"vc_ld_page": 4}, "cache must not be null")])
 def test_attention_refuses(change, message):

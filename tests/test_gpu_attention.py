@@ -165,9 +165,9 @@ def test_the_hints_steer_only_the_split(seqs):
     b.check(b.layer()(b.q, b.cache, b.table, b.kv_lens, b.q_begin))
 
 
-@pytest.mark.parametrize("std,scale", [(30.0, None), (1.5, 3.0), (1.5, 0.0), (1.5, -0.1)])
+@pytest.mark.parametrize("std,scale", [(30.0, None), (1.5, 3.0), (1.5, 0.0)])
 @pytest.mark.parametrize("seqs", [[(1, 3000)], [(5, 500)], [(300, 700)]])
-def test_peaked_flat_and_turned_scores(std, scale, seqs):
+def test_peaked_and_flat_scores(std, scale, seqs):
     b = Batch(seqs, 8, 2, 128, 64, std=std)
     lse = torch.empty(b.q.shape[0], 8, device="cuda")
     b.check(b.run(scale=scale, lse=lse), lse, scale)
