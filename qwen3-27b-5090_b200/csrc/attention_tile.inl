@@ -323,8 +323,9 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   if (warp >= C::kSoftmaxWarps) {
   if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
   // (the other warps are idle: they complete the warpgroup)
-  if (warp == C::kSoftmaxWarps + NT) {
-    // ---- copies -----------------------------------------------------------------------------------------------------------
+  if (warp == C::kSoftmaxWarps + NT || warp == C::kSoftmaxWarps + NT + 1) {
+    // ---- copies: two warps issue every other ring slot each (one would spend longer on it than the products take) --------------
+    const int turn_of = warp - C::kSoftmaxWarps - NT;
     const int boxes = C::kKeys / box, page_bits = __ffs(p.page_size) - 1;  // boxes per tile: at most eight, one per lane
     int slot = 0, issued = 0;
     uint32_t phase = 0;
@@ -356,6 +357,11 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
         constexpr int kBlocks = D / 64;
         const int d0 = C::kParts == 2 && !values ? part * kBlocks / 2 : 0, dn = C::kParts == 2 && !values ? kBlocks / 2 : kBlocks;
         const int rows = C::kParts == 2 && values ? C::kKeys / 2 : C::kKeys;
+        if ((issued & 1) != turn_of) {  // the other warp's
+          issued++;
+          if (++slot == C::kSlots) slot = 0, phase ^= 1u;
+          continue;
+        }
         if (issued >= C::kSlots && !warp_wait(empty(slot), phase ^ 1u, &abort_flag, status, kStatusEmptyWaitTimeout, 0)) {
           stop = true;
           return;
@@ -395,6 +401,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       }
     if (stop)  // unwinding: no copy may still be in flight when the CTA ends
       for (int s = 0; s < C::kSlots && s < issued; s++) {
+        if ((s & 1) != turn_of) continue;  // (the number of slots is even)
         const int last = issued - 1 - ((issued - 1 - s) % C::kSlots + C::kSlots) % C::kSlots;  // last use of slot s
         uint32_t unused = 0;
         if (lane == 0) mbar_wait_bounded(full(s), uint32_t(last / C::kSlots) & 1u, &abort_flag, &unused, kStatusDrainTimeout);
