@@ -23,8 +23,7 @@ struct TileCfg {
   static constexpr int kRows = 128 * kTiles;
   static constexpr int kKeys = 128;
   // What a segment costs beside its tiles (Q, the start and the end of the pipeline, the epilogue), in tiles: it counts in the shares
-  static constexpr int kSegmentCost = 3;
-  static constexpr int kPolyEvery = 3;                           // every third pair's exponentials on the FMA units
+  static constexpr int kSegmentCost = 5;
   static constexpr int kParts = D == 256 ? 2 : 1;                // ring slots per K or V tile
   static constexpr int kSlotBytes = kKeys * D * 2 / kParts;
   static constexpr int kSlots = D == 64 ? 8 : 4;
@@ -128,20 +127,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
-}
-// 2^x of two values on the FMA units (x <= 8; below -126 as -126): x = n + r with n the nearest integer, 2^r by a polynomial of
-// degree 5 in r (fitted on [-1/2, 1/2] for the smallest relative error, 1 at 0: 2^-22 in fp32 arithmetic), n added to its exponent.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  const float2 magic = make_float2(12582912.f, 12582912.f), unmagic = make_float2(-12582912.f, -12582912.f), minus = make_float2(-1.f, -1.f);
-  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  const float2 t = add2(x, magic);  // 1.5 2^23 + n: n in the low bits
-  const float2 r = fma2(add2(t, unmagic), minus, x);
-  float2 e = fma2(r, make_float2(1.326472731307149e-3f, 1.326472731307149e-3f), make_float2(9.671512991189957e-3f, 9.671512991189957e-3f));
-  e = fma2(e, r, make_float2(5.550733581185341e-2f, 5.550733581185341e-2f));
-  e = fma2(e, r, make_float2(0.24022242426872253f, 0.24022242426872253f));
-  e = fma2(e, r, make_float2(0.6931470036506653f, 0.6931470036506653f));
-  e = fma2(e, r, make_float2(1.f, 1.f));
-  return make_float2(__int_as_float((__float_as_int(t.x) << 23) + __float_as_int(e.x)), __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(e.y)));
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -644,8 +629,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
 #pragma unroll
               for (int x = 0; x < 16; x++) {
                 float2 e = fma2(make_float2(s[2 * x], s[2 * x + 1]), scale2, off2);
-                // the special-function units alone would need as long as the products: some of the pairs go through the FMA units
-                e = x % C::kPolyEvery == 1 ? exp2_poly(e) : make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
                 sum[x & 1] = add2(sum[x & 1], e);
                 T2 v;
                 narrow(e, &v);
@@ -696,7 +680,6 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
           half_l[half][tile][row_in_tile] = l;
           pair_bar();
           l += half_l[half ^ 1][tile][row_in_tile];
-          if (m == -INFINITY) l = 0.f;  // (a row that sees nothing: its 2^-126s are not sums)
           const bool whole = from == 0 && end == cur.r.tiles, live = row < cur.rows && done;
           const float inv = l == 0.f ? 0.f : 1.f / l;
           uint16_t* out = static_cast<uint16_t*>(p.out) + (cur.s.row0 + row / G) * p.out_ld_token + (cur.hk * G + row % G) * p.out_ld_head + half * (D / 2);
