@@ -14,7 +14,9 @@ import sys
 import torch
 
 from . import layouts, weights
+from .attention import Attention, KvCache
 from .q27lib import call, lib
+from .rotary import Rotary, qk_norm_rope, rope
 
 SKINNY_MAX_M = 128  # rows up to which the weight-streaming kernel is used (the reference: 64)
 # The reference shares one 32 MiB workspace (engine/src/model.h:462), enough here for every shape of the model up to
@@ -221,3 +223,52 @@ class Fp4Mlp:
             call("q27b_silu_mul_quant_fp4_glu", gbuf, M, gu.out, self.alpha_gate, self.alpha_up, dn.in_scale, hq.q, hq.sf, s)
         dn.gemm(M, hq.q, hq.sf, out, residual)
         return out
+
+
+class Fp4Attention:
+    """The attention of one layer between its NVFP4 projections, o(attention(q, k, v)) (+ residual), beside Fp4Mlp: the q | k | v
+    projections of x, per-head norm and rotation of queries and keys with the write of keys and values into the paged cache,
+    attention over the cache, the output projection.
+
+    * few rows (M <= 128): one weight-streaming launch over the stacked q | k | v rows, one alpha each;
+    * many rows: the three projections one after the other (the many-row GEMM takes one alpha), on views of the same weights.
+    """
+
+    def __init__(self, q: Fp4Linear, k: Fp4Linear, v: Fp4Linear, o: Fp4Linear, head_dim: int, rotary: Rotary, q_norm: torch.Tensor | None = None,
+                 k_norm: torch.Tensor | None = None, eps: float = 1e-6, window: int | None = None, sinks: int = 0, scale: float | None = None):
+        assert (q_norm is None) == (k_norm is None) and q.rows() == o.inp and k.rows() == v.rows()
+        assert q.rows() % head_dim == 0 and k.rows() % head_dim == 0 and q.inp == k.inp == v.inp
+        self.heads, self.kv_heads, self.head_dim = q.rows() // head_dim, k.rows() // head_dim, head_dim
+        self.qkv, self.o, self.rotary, self.q_norm, self.k_norm, self.eps = Fp4Linear.fused([q, k, v]), o, rotary, q_norm, k_norm, eps
+        self.attention = Attention(self.heads, self.kv_heads, head_dim, window, sinks, scale)
+        row, at = 0, 0
+        self.parts = []
+        for p in (q, k, v):  # the same weights, part by part
+            part = Fp4Linear(self.qkv.w[row:row + p.rows()], self.qkv.sf[at:at + p.sf.numel()], p.w_scale2, self.qkv.in_scale, p.rows(), p.inp, False, q.ws)
+            self.parts.append(part)
+            row, at = row + p.rows(), at + p.sf.numel()
+
+    def __call__(self, x: torch.Tensor, positions: torch.Tensor, cache: KvCache, slots: torch.Tensor, table: torch.Tensor, kv_lens: torch.Tensor,
+                 q_begin: torch.Tensor | None = None, max_new: int | None = None, max_kv: int | None = None,
+                 residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """x: bf16 / fp32 [M][hidden], the newest tokens of the batch; positions, slots [M]: of each token, and its place in the
+        cache; table, kv_lens (with the new tokens), q_begin, max_new, max_kv: as Attention takes them. Returns fp32 [M][hidden]
+        (+ residual, which may be `out`). Rows in no sequence come back undefined."""
+        M = x.shape[0]
+        if M == 0:
+            return torch.empty(0, self.o.rows(), dtype=torch.float32, device=x.device) if out is None else out
+        if M <= SKINNY_MAX_M:
+            rows = self.qkv(x).unflatten(1, (-1, self.head_dim))
+            q, k, v = rows.split([self.heads, self.kv_heads, self.kv_heads], 1)
+        else:
+            codes, sf = self.qkv._scratch(M).quantize(x, self.qkv.in_scale)
+            q, k, v = (torch.empty(M, p.rows(), dtype=torch.bfloat16, device=x.device) for p in self.parts)
+            for p, y in zip(self.parts, (q, k, v)):
+                p.gemm(M, codes, sf, y)
+            q, k, v = (y.unflatten(1, (-1, self.head_dim)) for y in (q, k, v))
+        if self.q_norm is None:
+            q = rope(self.rotary, positions, q, k, v=v, cache=cache, slots=slots)
+        else:
+            q = qk_norm_rope(self.rotary, positions, q, k, self.q_norm, self.k_norm, self.eps, v=v, cache=cache, slots=slots)
+        y = self.attention(q, cache, table, kv_lens, q_begin, max_new, max_kv)
+        return self.o(y.flatten(1), out, torch.float32, residual)

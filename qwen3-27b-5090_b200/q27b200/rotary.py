@@ -118,14 +118,20 @@ def _launch(what, rotary, positions, q, k, v, q_out, k_out, q_weight, k_weight, 
 
 
 def rope(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
-         k_out: torch.Tensor | None = None):
+         k_out: torch.Tensor | None = None, v: torch.Tensor | None = None, cache=None, slots: torch.Tensor | None = None):
     """Rotates q [T, heads, D] (and k [T, kv_heads, D]) by positions [T]; returns (q_out, k_out). The outputs may be the inputs
-    themselves; without them new tensors of the inputs' type are made."""
-    q_out = _new(q, q.dtype) if q_out is None else q_out
-    if k is not None and k_out is None:
+    themselves; without them new tensors of the inputs' type are made. With a cache (attention.KvCache) k, and v as it is, go to
+    its places slots [T] as in qk_norm_rope, the outputs have its type, and q_out alone is returned."""
+    if cache is not None and (k is None or k_out is not None):
+        raise ValueError("rope: with a cache k goes into it, and nowhere else")
+    if cache is None and (v is not None or slots is not None):
+        raise ValueError("rope: v and slots need a cache")
+    if q_out is None:
+        q_out = _new(q, q.dtype if cache is None else cache.dtype)
+    if k is not None and k_out is None and cache is None:
         k_out = _new(k, q_out.dtype)
-    _launch("rope", rotary, positions, q, k, None, q_out, k_out, None, None, 0.0, False, None, None)
-    return q_out, k_out
+    _launch("rope", rotary, positions, q, k, v, q_out, k_out, None, None, 0.0, False, cache, slots)
+    return (q_out, k_out) if cache is None else q_out
 
 
 def qk_norm_rope(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
