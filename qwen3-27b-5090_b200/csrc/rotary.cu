@@ -13,7 +13,11 @@
 //
 // Bound: memory (every value is read and written once). Shape: a CTA takes a few tokens; its threads first compute the
 // (token, pair) table of cos and sin once into shared memory - not once per head, which would cost more instructions
-// than the loads leave room for - and then walk the tokens' head rows, D / 8 lanes to a row, 8 channels (4 pairs) to a lane.
+// than the loads leave room for - and then walk the tokens' head rows, D / 16 lanes to a row, 16 channels (8 pairs) to a lane,
+// the next row's loads in flight. Measured: 8191 tokens of 28 heads x 256 channels (fp16): 43 us, 5.5 TB/s (84 % of the measured
+// copy rate); 4096 tokens of 40 + 8 + 8 heads x 128 channels with the norm into the cache: 26 us, 4.5 TB/s (its 1024 CTAs
+// are 1.7 waves of the GPU); with 8 channels to a lane 60 and 44 us; with three or five CTAs per SM instead of four 48 and
+// 51, 31 and 33 us; with one token per CTA instead of four 64 and 46 us.
 //
 // Programmatic dependent launch: as every kernel of this library, wait for the predecessor first, release the successor
 // only then.
