@@ -365,7 +365,9 @@ int q27b_qk_norm_rope(const q27b_qk_rope* args, void* stream);
  * newest of them. The token at position p sees the positions j <= p with j > p - window (window > 0) or j < sinks; a token
  * that sees nothing (a negative position: more rows than tokens) gives zeros and an lse of -infinity. Rows of q in no
  * sequence are left as they were. Pages that no row sees are never read and may hold any table entry; what lies in
- * the cache behind a sequence's end is never used, whatever it holds. Strides in elements; channels contiguous; bases
+ * the cache behind a sequence's end is never used, whatever it holds. A query or a key that is not finite reaches only the
+ * rows that use it; a VALUE that is not finite may also reach rows of the same call that the mask hides it from, if another
+ * row of their sequence sees it (0 x infinity, as in a dense softmax(S) V). Strides in elements; channels contiguous; bases
  * 16-byte aligned and strides multiples of 8 elements. Lengths, tables and rows may change between replays of a captured
  * launch: the kernels read them on the device. A table entry that a row needs but that lies outside the cache, or a length
  * past the table, reads nothing and raises device status 10. */
