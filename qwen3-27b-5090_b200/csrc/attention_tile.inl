@@ -19,14 +19,15 @@
 // Roles: eight warps per row tile (softmax, scaling, epilogue, and the load of the next segment's Q), a warp per row tile that issues
 // its products, two warps that issue the copies. K and V pass through one ring in the order in which the products use them.
 //
-// What bounds it: per pair of row tiles and 128 keys the products need 2048 cycles and the exponentials as many; measured are 3700.
-// The rest is the chain from S over the softmax (1900 cycles, two thirds of them exponentials and their conversions while both
-// tiles compete for the special-function units) to P V and the next S (1100 and the signals between the warps). Measured on
-// 8192 tokens, 40 heads over 8 of 128 channels, bf16, causal: 735 us, 936 TFLOP/s (57 % of the measured burst rate of a
-// matrix product, 67 % of the sustained one; the power limit holds the clock at 1.5 to 1.7 GHz); 512 tokens behind 24000 of
-// 256 channels: 285 us, 1070 TFLOP/s. Tried and measured worse or equal: one thread per row (790 us), 64-key tiles with two S
-// buffers (1470 us: the cost per tile hardly depends on its size), a third of the exponentials as a polynomial on the FMA units
-// (no difference), both tiles' products issued by one warp in fixed order (820 us) or by two in strict turns (766 us).
+// What bounds it: per pair of row tiles and 128 keys the products need 2048 cycles and the exponentials as many (a quarter less
+// with those on the FMA units); measured are 3500. The rest is the chain from S over the softmax (1900 cycles, more than half of
+// them exponentials and their conversions while both tiles compete for the same units) to P V and the next S (1100 and the signals
+// between the warps). Measured on 8192 tokens, 40 heads over 8 of 128 channels, bf16, causal: 700 us, 980 TFLOP/s (60 % of the
+// measured burst rate of a matrix product, 70 % of the sustained one; the power limit holds the clock at 1.5 to 1.7 GHz, and
+// after seconds of load 800 us are measured); 512 tokens behind 24000 of 256 channels: 285 us, 1070 TFLOP/s. Tried and measured
+// worse or equal: one thread per row (790 us against 766 at the time), 64-key tiles with two S buffers (1470 against 790: the cost
+// per tile hardly depends on its size), both tiles' products issued by one warp in fixed order (820) or by two in strict turns
+// (766 against 735), the two row tiles sharing a short segment's keys (no gain for verification).
 
 template <int D>
 struct TileCfg {
@@ -35,6 +36,10 @@ struct TileCfg {
   static constexpr int kKeys = 128;
   // What a segment costs beside its tiles (Q, the start and the end of the pipeline, the epilogue), in tiles: it counts in the shares
   static constexpr int kSegmentCost = 5;
+  // Whether pair x of a thread's exponentials goes through the FMA units: every fourth where two row tiles compete for the
+  // special-function units (prompt of 8192: 733 -> 700 us; every third to sixth alike), none at 256 channels, where the products
+  // take twice as long (chunk of 512: 285 us without, 301 with).
+  static constexpr bool on_fma(int x) { return D != 256 && x % 4 == 1; }
   static constexpr int kParts = D == 256 ? 2 : 1;                // ring slots per K or V tile
   static constexpr int kSlotBytes = kKeys * D * 2 / kParts;
   static constexpr int kSlots = D == 64 ? 8 : 4;
@@ -138,6 +143,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
+}
+// 2^x of two values on the FMA units (x <= 8; below -126 as -126): x = n + r with n the nearest integer, 2^r by a polynomial of
+// degree 5 in r (fitted on [-1/2, 1/2] for the smallest relative error, 1 at 0: 2^-22 in fp32 arithmetic), n added to its exponent.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f), unmagic = make_float2(-12582912.f, -12582912.f), minus = make_float2(-1.f, -1.f);
+  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const float2 t = add2(x, magic);  // 1.5 2^23 + n: n in the low bits
+  const float2 r = fma2(add2(t, unmagic), minus, x);
+  float2 e = fma2(r, make_float2(1.326472731307149e-3f, 1.326472731307149e-3f), make_float2(9.671512991189957e-3f, 9.671512991189957e-3f));
+  e = fma2(e, r, make_float2(5.550733581185341e-2f, 5.550733581185341e-2f));
+  e = fma2(e, r, make_float2(0.24022242426872253f, 0.24022242426872253f));
+  e = fma2(e, r, make_float2(0.6931470036506653f, 0.6931470036506653f));
+  e = fma2(e, r, make_float2(1.f, 1.f));
+  return make_float2(__int_as_float((__float_as_int(t.x) << 23) + __float_as_int(e.x)), __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(e.y)));
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -639,7 +658,8 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
 #pragma unroll
               for (int x = 0; x < 16; x++) {
                 float2 e = fma2(make_float2(s[2 * x], s[2 * x + 1]), scale2, off2);
-                e = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                // the special-function units alone would need as long as the products: some of the pairs go through the FMA units
+                e = C::on_fma(x) ? exp2_poly(e) : make_float2(exp2_fast(e.x), exp2_fast(e.y));
                 sum[x & 1] = add2(sum[x & 1], e);
                 T2 v;
                 narrow(e, &v);
@@ -690,6 +710,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
           half_l[half][tile][row_in_tile] = l;
           pair_bar();
           l += half_l[half ^ 1][tile][row_in_tile];
+          if (m == -INFINITY) l = 0.f;  // (a row that sees nothing: the polynomial's 2^-126s are no sum)
           const bool whole = from == 0 && end == cur.r.tiles, live = row < cur.rows && done;
           const float inv = l == 0.f ? 0.f : 1.f / l;
           uint16_t* out = static_cast<uint16_t*>(p.out) + (cur.s.row0 + row / G) * p.out_ld_token + (cur.hk * G + row % G) * p.out_ld_head + half * (D / 2);
