@@ -634,6 +634,7 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
             if (rarely(__any_sync(0xffffffffu, grow))) {
               const float f = grow ? exp2_fast((m - tile_m) * scale_log2) : 1.f;  // (m = -infinity: 0)
               if (grow) m = tile_m, mc = m * scale_log2, l *= f;
+              if (mc == INFINITY) mc = NAN;  // an infinite score: infinity - infinity, for the polynomial's pairs too
               if (i > from) {
                 if (NT == 1) wait_pv();
 #pragma unroll

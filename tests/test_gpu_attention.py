@@ -212,6 +212,19 @@ def test_non_finite_queries_and_masked_keys(seqs):
             at += new
 
 
+@pytest.mark.parametrize("seqs", [[(1, 700), (1, 64)], [(4, 700), (2, 100)], [(150, 700), (90, 90)]])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_an_infinite_or_nan_score_makes_the_row_nan(seqs, D, bad):
+    """At every place of a tile, whichever way its exponential is taken: one key of the first sequence, seen by all its rows."""
+    for j in (0, 1, 2, 3, 5, 37, 66, 127, 130, 300):
+        b = Batch(seqs, 4, 2, D, 64)
+        b.q.abs_()
+        b.cache.k[b.table[0, j // 64].long(), :, j % 64] = bad
+        out = b.run()
+        assert bool(out[:seqs[0][0]].isnan().all()) and bool(out[seqs[0][0]:].isfinite().all()), j
+
+
 def test_offsets_past_32_bits():
     """A cache of more than 2^31 elements (one tensor for keys and values), sequences in its last pages."""
     D, page, Hk = 128, 64, 8
