@@ -10,7 +10,7 @@ import struct
 
 import torch
 
-from .q27lib import call
+from .q27lib import call, last_error, lib
 
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # Q27B_F32, Q27B_BF16, Q27B_F16
@@ -30,15 +30,21 @@ def device_of(what: str, *tensors: torch.Tensor) -> torch.device:
     return dev
 
 
+_entries: dict = {}
+
+
 def launch(name: str, packed: bytes, dev: torch.device):
     """The C entry on the device's current stream; the device is made current for the call where it is not."""
     index = dev.index
-    if index == torch.cuda.current_device():
-        # (the raw handle: making a Stream object of it costs as much as the launch)
-        call(name, packed, torch._C._cuda_getCurrentRawStream(index))
-    else:
+    if index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            call(name, packed, torch._C._cuda_getCurrentRawStream(index))
+            return launch(name, packed, dev)
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(lib(), name)
+    # (the raw handle: making a Stream object of it costs as much as the launch)
+    if fn(packed, torch._C._cuda_getCurrentRawStream(index)):
+        raise RuntimeError(f"{name}: {last_error()}")
 
 
 class Rotary:
@@ -61,37 +67,45 @@ class Rotary:
         self.turns_ptr = self.turns.data_ptr()
 
 
-def _heads(what: str, x: torch.Tensor, T: int, heads: int, D: int):
+def _heads(what: str, x: torch.Tensor, shape):
     """Base and strides of [T, heads, D] with contiguous channels."""
-    if x.shape != (T, heads, D):
-        raise ValueError(f"{what}: expected [{T}, {heads}, {D}], got {list(x.shape)}")
+    if x.shape != shape:
+        raise ValueError(f"{what}: expected {list(shape)}, got {list(x.shape)}")
     a, b, c = x.stride()
-    if c != 1 and D > 1:
+    if c != 1 and shape[2] > 1:
         raise ValueError(f"{what}: the channels of a head must be contiguous")
     return x.data_ptr(), a, b
 
 
-def _new(like: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
-
-
-def _launch(what, rotary, positions, q, k, v, q_out, k_out, q_weight, k_weight, eps, zero_centred, cache, slots):
+def _launch(what, rotary, positions, q, k, v, q_out, k_out, q_weight, k_weight, eps, zero_centred, cache, slots, out_dtype):
+    """Checks, outputs where none are given (of out_dtype), and the launch."""
     if q.dim() != 3 or (k is not None and k.dim() != 3):
         raise ValueError(f"{what}: q and k must be [tokens, heads, channels]")
-    T, Hq, D = q.shape
+    shape = q.shape
+    T, Hq, D = shape
     dev = device_of(what, q, positions, rotary.turns, k, v, q_out, k_out, q_weight, k_weight, slots, cache.k if cache else None)
-    dtype, out_dtype, pos_dtype = q.dtype, q_out.dtype, positions.dtype
-    if dtype not in DTYPES or out_dtype not in DTYPES:
+    dtype, pos_dtype = q.dtype, positions.dtype
+    if q_out is not None:
+        out_dtype = q_out.dtype
+    in_code, out_code = DTYPES.get(dtype), DTYPES.get(out_dtype)
+    if in_code is None or out_code is None:
         raise ValueError(f"{what}: inputs and outputs must be fp32, bf16 or fp16, got {dtype} and {out_dtype}")
-    if (pos_dtype is not torch.int64 and pos_dtype is not torch.int32) or positions.shape != (T,) or not positions.is_contiguous():
+    pos64 = pos_dtype is torch.int64
+    if not (pos64 or pos_dtype is torch.int32) or positions.shape != (T,) or not positions.is_contiguous():
         raise ValueError(f"{what}: positions must be int64 or int32 [{T}], contiguous")
-    qp, qo = _heads(what + ": q", q, T, Hq, D), _heads(what + ": q_out", q_out, T, Hq, D)
+    qp = _heads(what + ": q", q, shape)
+    if q_out is None:
+        q_out = torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
+        qo = (q_out.data_ptr(), Hq * D, D)
+    else:
+        qo = _heads(what + ": q_out", q_out, shape)
     Hk, kp, vp, ko = 0, _NONE3, _NONE3, _NONE3
     if k is not None:
         Hk = k.shape[1]
-        kp = _heads(what + ": k", k, T, Hk, D)
+        k_shape = (T, Hk, D)
+        kp = _heads(what + ": k", k, k_shape)
         if v is not None:
-            vp = _heads(what + ": v", v, T, Hk, D)
+            vp = _heads(what + ": v", v, k_shape)
         if k.dtype is not dtype or (v is not None and v.dtype is not dtype):
             raise ValueError(f"{what}: q, k and v must have one type")
     qw = kw = 0
@@ -109,12 +123,17 @@ def _launch(what, rotary, positions, q, k, v, q_out, k_out, q_weight, k_weight, 
             raise ValueError(f"{what}: the cache holds {cache.kv_heads} heads of {cache.head_dim} channels in {cache.dtype}, got {Hk} of {D} for {out_dtype}")
         slot_ptr, page_size, pages, kc, vc = slots.data_ptr(), cache.page_size, cache.pages, cache.k_packed, cache.v_packed
     elif k is not None:
-        ko = _heads(what + ": k_out", k_out, T, Hk, D)
-        if k_out.dtype is not out_dtype:
-            raise ValueError(f"{what}: q_out and k_out must have one type")
+        if k_out is None:
+            k_out = torch.empty_like(k, dtype=out_dtype, memory_format=torch.contiguous_format)
+            ko = (k_out.data_ptr(), Hk * D, D)
+        else:
+            ko = _heads(what + ": k_out", k_out, k_shape)
+            if k_out.dtype is not out_dtype:
+                raise ValueError(f"{what}: q_out and k_out must have one type")
     launch("q27b_qk_norm_rope", QK_ROPE.pack(
-        T, Hq, Hk, D, rotary.rot_dim, rotary.interleaved, DTYPES[dtype], DTYPES[out_dtype], pos_dtype is torch.int64, weight_f32, zero_centred, eps,
+        T, Hq, Hk, D, rotary.rot_dim, rotary.interleaved, in_code, out_code, pos64, weight_f32, zero_centred, eps,
         rotary.amplitude, positions.data_ptr(), rotary.turns_ptr, qw, kw, *qp, *kp, *vp, *qo, *ko, slot_ptr, page_size, pages, *kc, *vc), dev)
+    return q_out, k_out
 
 
 def rope(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
@@ -126,12 +145,8 @@ def rope(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Tens
         raise ValueError("rope: with a cache k goes into it, and nowhere else")
     if cache is None and (v is not None or slots is not None):
         raise ValueError("rope: v and slots need a cache")
-    if q_out is None:
-        q_out = _new(q, q.dtype if cache is None else cache.dtype)
-    if k is not None and k_out is None and cache is None:
-        k_out = _new(k, q_out.dtype)
-    _launch("rope", rotary, positions, q, k, v, q_out, k_out, None, None, 0.0, False, cache, slots)
-    return (q_out, k_out) if cache is None else q_out
+    out = _launch("rope", rotary, positions, q, k, v, q_out, k_out, None, None, 0.0, False, cache, slots, q.dtype if cache is None else cache.dtype)
+    return out if cache is None else out[0]
 
 
 def qk_norm_rope(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -147,9 +162,6 @@ def qk_norm_rope(rotary: Rotary, positions: torch.Tensor, q: torch.Tensor, k: to
         raise ValueError("qk_norm_rope: v and slots need a cache")
     if q_weight is None or k_weight is None or k is None:
         raise ValueError("qk_norm_rope: k and both weights are needed (rope rotates without the norm)")
-    if q_out is None:
-        q_out = _new(q, cache.dtype if cache is not None else dtype or q.dtype)
-    if cache is None and k_out is None:
-        k_out = _new(k, q_out.dtype)
-    _launch("qk_norm_rope", rotary, positions, q, k, v, q_out, k_out, q_weight, k_weight, float(eps), zero_centred, cache, slots)
-    return q_out if cache is not None else (q_out, k_out)
+    out = _launch("qk_norm_rope", rotary, positions, q, k, v, q_out, k_out, q_weight, k_weight, float(eps), zero_centred, cache, slots,
+                  cache.dtype if cache is not None else dtype or q.dtype)
+    return out if cache is None else out[0]
