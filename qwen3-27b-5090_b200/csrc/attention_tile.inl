@@ -243,7 +243,6 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
     prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
   }
   pdl_wait();
-  pdl_trigger();
 
   // ---- this CTA's range of the tiles: every warp sums a run of sequences, its lanes share a sequence's segments ---------------
   const int G = p.heads / p.kv_heads, run = (p.B + kWarps - 1) / kWarps, b_lo = min(warp * run, p.B), b_hi = min(b_lo + run, p.B);
@@ -314,6 +313,9 @@ __global__ void __launch_bounds__(TileCfg<D>::kThreads, 1)
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  // Only now: a successor that starts early beside this CTA and takes tensor memory of its own before it waits for this kernel
+  // would hold what this CTA still had to take.
+  pdl_trigger();
   const uint32_t tmem = tmem_word;
   TileCursor cur;
   cur.b = start_b;

@@ -307,6 +307,21 @@ def test_bad_pages_and_lengths_are_reported():
         assert device_status() == 0
 
 
+@pytest.mark.parametrize("new", [1, 5, 100])
+@pytest.mark.parametrize("heads,kv_heads,D", [(4, 1, 128), (6, 2, 256), (3, 1, 64)])
+def test_a_cache_of_one_page_and_pages_shared_by_sequences(new, heads, kv_heads, D):
+    b = Batch([(new, 128)], heads, kv_heads, D, 128, spare=0)
+    assert b.cache.pages == 1
+    want = b.run()
+    b.check(want)
+    # two sequences over the same pages, one of them a token shorter
+    both = b.layer()(torch.cat([b.q, b.q]), b.cache, b.table.expand(2, -1), torch.tensor([128, 127], dtype=torch.int32, device="cuda"),
+                     torch.tensor([0, new, 2 * new], dtype=torch.int32, device="cuda"), new)
+    b.check(both[:new])
+    o, _, bound, _ = attention64(b.q, b.keys[0][:127], b.values[0][:127], new, 127, 0, 0, D ** -0.5)
+    assert bool(((both[new:].double() - o).abs() <= bound).all())
+
+
 def test_nothing_to_do():
     b = Batch([(1, 10)], 4, 2, 64, 16)
     layer = b.layer()
